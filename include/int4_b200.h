@@ -280,6 +280,87 @@ int i4b_silu_mul(const void* gate_up, void* y, int64_t B, int64_t I, void* strea
 /* out[r] = index of the first maximum of bf16 row x[r, 0..n) (greedy decoding, as torch.argmax). */
 int i4b_argmax_rows(const void* x, int64_t rows, int64_t n, int64_t* out, void* stream);
 
+/* ---- Serving over a paged key-value cache (bf16 or fp16, head_dim 64 or 128) ----
+ *
+ * Sequences of different lengths, each with its positions in fixed-size pages that a block table names, next to the
+ * one-position calls above.  No counterpart in the reference, whose decode benchmark runs one batch at one position
+ * over transformers' StaticCache (benchmarks/eval_llama.py:121-183).  A position's slot is its index in the sequence's
+ * pages (its rotary angle is a matter of i4b_paged_kv_append alone, so slots may be compacted).
+ *
+ * Element (page, head, token, d) of the keys is at k + page * k_stride_page + head * k_stride_head +
+ * token * k_stride_token + d, the same with v; strides are in elements and multiples of 8, bases 16-byte aligned, so
+ * both [pages, kv_heads, page_size, head_dim] and [pages, page_size, kv_heads, head_dim] memory will do.
+ * block_table[seq * table_stride + i] is the page of slots i * page_size ...; an entry outside [0, num_pages) that a
+ * length reaches is a page that holds nothing: its slots are left out of the attention, and nothing is written there.
+ * page_size: a multiple of 8.  seqs <= 4096.  max_pages * page_size < 2^31 - 64.
+ * All indices and lengths are device int32, so the calls can be captured in a CUDA graph.  Lengths are read as
+ * clamped to [0, max_pages * page_size]. */
+typedef struct i4b_paged_cache {
+  void* k;
+  void* v;
+  int64_t k_stride_page, k_stride_head, k_stride_token;
+  int64_t v_stride_page, v_stride_head, v_stride_token;
+  const int32_t* block_table; /* [seqs, max_pages], unit stride along the pages */
+  int64_t table_stride;
+  int64_t num_pages, kv_heads, page_size, head_dim;
+  int64_t seqs, max_pages;
+  int32_t dtype; /* I4B_BF16 or I4B_F16: keys, values, queries and outputs */
+} i4b_paged_cache;
+
+/* Rotary embedding of `tokens` tokens and their keys and values written into pages.  qkv row i (rows stride_qkv
+ * elements apart, a multiple of 8, 16-byte aligned) holds the q, k and v heads of token i; cos / sin [max_pos,
+ * head_dim] contiguous, of the cache's dtype or I4B_F32 (table_dtype), 16-byte aligned.  Token i has its angle from
+ * row positions[i] and goes to slot slots[i] of sequence seqs[i] (seqs NULL: sequence i).  q_out[tokens, nq, head_dim]
+ * receives the rotated queries.  t * cos + rotate_half(t) * sin is computed in fp32 and rounded once
+ * (i4b_rope_kv_cache rounds each product too, as transformers does).  A slot or sequence outside the table writes
+ * nothing to the cache (padding); a position outside the tables gives a zero query and writes nothing.  Two tokens of
+ * one call must not name the same slot of the same sequence. */
+int i4b_paged_kv_append(const i4b_paged_cache* cache, const void* qkv, int64_t stride_qkv, int64_t tokens, int64_t nq,
+                        const void* cos_table, const void* sin_table, int table_dtype, int64_t max_pos,
+                        const int32_t* positions, const int32_t* slots, const int32_t* seqs, void* q_out, void* stream);
+
+/* Bytes of workspace i4b_paged_decode_attention needs (0: sizes not supported, or no B200).  Needs no clearing; calls
+ * that share a workspace must not overlap in time. */
+size_t i4b_paged_attention_workspace_size(int64_t seqs, int64_t nq, int64_t kv_heads, int64_t head_dim,
+                                          int64_t capacity, int with_weights);
+
+/* out[seqs, nq, head_dim] = softmax(q . K^T * scale) . V over slots 0..lens[b]-1 of each sequence, query head h reading
+ * kv head h / (nq / kv_heads); zeros where no slot is left.  fp32 softmax; the probabilities are rounded to the cache's
+ * type for the product with V.  q: element (b, h, d) at q + b * stride_qb + h * stride_qh + d, strides multiples of 8,
+ * 16-byte aligned.  weights, when not NULL: fp32, weights[b * stride_wb + kvh * stride_wh + j] += the probability of
+ * slot j summed over the query heads of kv head kvh, j < lens[b]; the rest is left as it was.  Results repeat bit by
+ * bit for the same lengths.  workspace: 16-byte aligned. */
+int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int64_t stride_qb, int64_t stride_qh,
+                               int64_t nq, const int32_t* lens, float scale, void* out, float* weights,
+                               int64_t stride_wb, int64_t stride_wh, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Keeps at most `budget` slots of every sequence and copies their keys and values, in order, into new pages.
+ * A sequence longer than the budget keeps, for each kv head by itself, its last `recent` slots and the budget - recent
+ * of largest weight among the others (ties: the lower slot; -0 as +0; NaN below everything); a shorter one keeps all.
+ * weights: fp32 [seqs, kv_heads, width] with strides, width >= max_pages * page_size.  new_table[seqs, >= budget /
+ * page_size rounded up] names the new pages, none of which may be a page that `cache` still reads in this call.
+ * new_lens[seqs] = min(lens, budget); kept[seqs, kv_heads, budget] (contiguous) = the slots kept, -1 behind the last;
+ * weights_out [seqs, kv_heads, width] = their weights, zeros behind the last (may be `weights` itself).
+ * 0 <= recent <= budget, budget >= 1. */
+int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t stride_wb, int64_t stride_wh,
+                    int64_t width, const int32_t* lens, const int32_t* new_table, int64_t new_table_stride,
+                    int64_t new_max_pages, int64_t budget, int64_t recent, int32_t* new_lens, int32_t* kept,
+                    float* weights_out, int64_t stride_ob, int64_t stride_oh, void* stream);
+
+/* Log probabilities of given tokens, with each row's entropy and most probable tokens, in one reading of the logits.
+ * x: row r at x + r * stride_x, n contiguous logits of dtype I4B_BF16, I4B_F16 or I4B_F32.
+ * logprobs[r] = x[r, targets[r]] - logsumexp(x[r]); a negative target (padding) gives 0, one >= n a NaN.
+ * entropy[r] = -sum p log p.  top_ids / top_logprobs [rows, top]: the `top` largest logits of the row in order, ties to
+ * the lower index, with their log probabilities (0 <= top <= I4B_MAX_TOP, top <= n; both may be NULL when top is 0).
+ * -inf logits have probability 0; a row of nothing else has log probabilities -inf and entropy 0.  A NaN or +inf makes
+ * the row's numbers NaN; a NaN logit is never among the alternatives (missing ones have id 0).  All in fp32.
+ * Replaces the log_softmax / cross entropy of the reference's eval_ppl (benchmarks/eval_llama.py:77-117). */
+#define I4B_MAX_TOP 32
+int i4b_token_logprobs(const void* x, int dtype, int64_t rows, int64_t n, int64_t stride_x, const int64_t* targets,
+                       int64_t top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                       void* stream);
+
 /* ---- Persistent decode of all decoder layers (one launch per token step) ----
  *
  * Replaces, for batch <= 8 single-token steps of a Llama-shaped W4A16 model on

@@ -554,6 +554,137 @@ int i4b_argmax_rows(const void* x, int64_t rows, int64_t n, int64_t* out, void* 
   return e == cudaSuccess ? I4B_OK : fail_cuda(e);
 }
 
+namespace {
+
+// The caller's description of a paged cache checked and brought into the kernels' form.
+int paged_cache(const i4b_paged_cache* in, PagedCache* c) {
+  if (!in) return I4B_ERR_INVALID_ARG;
+  if (in->dtype != I4B_BF16 && in->dtype != I4B_F16) return I4B_ERR_INVALID_ARG;
+  if (in->head_dim != 64 && in->head_dim != 128) return I4B_ERR_SHAPE;
+  if (in->page_size <= 0 || in->page_size % 8 != 0 || in->kv_heads <= 0 || in->kv_heads > 65535) return I4B_ERR_SHAPE;
+  if (in->num_pages <= 0 || in->num_pages > INT32_MAX || in->max_pages < 0 || in->seqs < 0 || in->seqs > 4096)
+    return I4B_ERR_SHAPE;
+  if (in->page_size > INT32_MAX - 64 || in->max_pages > (INT32_MAX - 64) / in->page_size) return I4B_ERR_SHAPE;
+  if (!in->k || !in->v || (!in->block_table && in->seqs * in->max_pages > 0)) return I4B_ERR_INVALID_ARG;
+  if (!aligned16(in->k) || !aligned16(in->v)) return I4B_ERR_LAYOUT;
+  int64_t st[] = {in->k_stride_page, in->k_stride_head, in->k_stride_token,
+                  in->v_stride_page, in->v_stride_head, in->v_stride_token};
+  const int64_t extent[] = {in->num_pages, in->kv_heads, in->page_size};
+  for (int i = 0; i < 6; ++i) {
+    if (extent[i % 3] == 1) st[i] = 0;  // never used: whatever the caller's view says
+    if (st[i] < 0 || st[i] % 8 != 0) return I4B_ERR_LAYOUT;
+  }
+  c->k = static_cast<uint16_t*>(in->k);
+  c->v = static_cast<uint16_t*>(in->v);
+  c->ks_page = st[0], c->ks_head = st[1], c->ks_token = st[2];
+  c->vs_page = st[3], c->vs_head = st[4], c->vs_token = st[5];
+  c->table = in->block_table;
+  c->table_stride = in->table_stride;
+  c->seqs = int(in->seqs);
+  c->capacity = int(in->max_pages * in->page_size);
+  c->num_pages = int(in->num_pages);
+  c->kv_heads = int(in->kv_heads);
+  c->head_dim = int(in->head_dim);
+  c->f16 = in->dtype == I4B_F16;
+  paged_set_page_size(c, int(in->page_size));
+  return I4B_OK;
+}
+
+}  // namespace
+
+int i4b_paged_kv_append(const i4b_paged_cache* cache, const void* qkv, int64_t stride_qkv, int64_t tokens, int64_t nq,
+                        const void* cos_table, const void* sin_table, int table_dtype, int64_t max_pos,
+                        const int32_t* positions, const int32_t* slots, const int32_t* seqs, void* q_out,
+                        void* stream) {
+  PagedCache c;
+  if (int st = paged_cache(cache, &c)) return st;
+  if (table_dtype != I4B_F32 && table_dtype != cache->dtype) return I4B_ERR_INVALID_ARG;
+  if (tokens < 0 || tokens > INT32_MAX || nq <= 0 || nq > 65535 || max_pos <= 0 || max_pos > INT32_MAX)
+    return I4B_ERR_SHAPE;
+  if (tokens == 0) return I4B_OK;
+  if (tokens == 1) stride_qkv = 0;  // never used
+  if (!qkv || !cos_table || !sin_table || !positions || !slots || !q_out) return I4B_ERR_INVALID_ARG;
+  if (!aligned16(qkv) || !aligned16(cos_table) || !aligned16(sin_table) || !aligned16(q_out) || stride_qkv % 8 != 0 ||
+      stride_qkv < 0)
+    return I4B_ERR_LAYOUT;
+  DevInfo d;
+  if (int st = current_device_info(&d)) return st;
+  const cudaError_t e = launch_paged_append(c, static_cast<const uint16_t*>(qkv), stride_qkv, tokens, cos_table, sin_table,
+                                            table_dtype == I4B_F32, int(max_pos), positions, slots, seqs,
+                                            static_cast<uint16_t*>(q_out), int(nq), static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? I4B_OK : fail_cuda(e);
+}
+
+size_t i4b_paged_attention_workspace_size(int64_t seqs, int64_t nq, int64_t kv_heads, int64_t head_dim,
+                                          int64_t capacity, int with_weights) {
+  if (seqs < 0 || seqs > 4096 || nq <= 0 || nq > 65535 || kv_heads <= 0 || nq % kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128) || capacity < 0 || capacity > INT32_MAX - 64)
+    return 0;
+  DevInfo d;
+  if (current_device_info(&d)) return 0;
+  return paged_attn_workspace(int(seqs), int(nq), int(head_dim), int(capacity), with_weights != 0, d.sms, nullptr, nullptr);
+}
+
+int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int64_t stride_qb, int64_t stride_qh,
+                               int64_t nq, const int32_t* lens, float scale, void* out, float* weights,
+                               int64_t stride_wb, int64_t stride_wh, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  PagedCache c;
+  if (int st = paged_cache(cache, &c)) return st;
+  if (nq <= 0 || nq > 65535 || nq % c.kv_heads != 0 || paged_attn_tiles(c, int(nq)) > INT32_MAX) return I4B_ERR_SHAPE;
+  if (c.seqs == 0) return I4B_OK;
+  if (!q || !lens || !out || !workspace) return I4B_ERR_INVALID_ARG;
+  if (c.seqs == 1) stride_qb = 0;  // never used
+  if (nq == 1) stride_qh = 0;
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || stride_qb < 0 || stride_qh < 0 || stride_qb % 8 != 0 || stride_qh % 8 != 0)
+    return I4B_ERR_LAYOUT;
+  DevInfo d;
+  if (int st = current_device_info(&d)) return st;
+  PagedAttnWorkspace w;
+  if (workspace_bytes < paged_attn_workspace(c.seqs, int(nq), c.head_dim, c.capacity, weights != nullptr, d.sms, workspace, &w))
+    return I4B_ERR_WORKSPACE;
+  const PagedAttn a = {static_cast<const uint16_t*>(q), stride_qb, stride_qh, lens, static_cast<uint16_t*>(out), int(nq),
+                       scale, weights, stride_wb, stride_wh};
+  const cudaError_t e = launch_paged_attn(c, a, w, d.sms, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? I4B_OK : fail_cuda(e);
+}
+
+int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t stride_wb, int64_t stride_wh,
+                    int64_t width, const int32_t* lens, const int32_t* new_table, int64_t new_table_stride,
+                    int64_t new_max_pages, int64_t budget, int64_t recent, int32_t* new_lens, int32_t* kept,
+                    float* weights_out, int64_t stride_ob, int64_t stride_oh, void* stream) {
+  PagedCache c;
+  if (int st = paged_cache(cache, &c)) return st;
+  if (width < c.capacity || width > INT32_MAX - 64 || budget < 1 || budget > INT32_MAX - 64 || recent < 0 ||
+      recent > budget || new_max_pages < (budget + c.page_size - 1) / c.page_size)
+    return I4B_ERR_SHAPE;
+  if (c.seqs == 0) return I4B_OK;
+  if (!lens || !new_table || !new_lens || !kept || (width > 0 && (!weights || !weights_out))) return I4B_ERR_INVALID_ARG;
+  DevInfo d;
+  if (int st = current_device_info(&d)) return st;
+  const PagedEvict p = {weights, stride_wb, stride_wh, lens, new_table, new_table_stride, int(budget), int(recent),
+                        int(width), new_lens, kept, weights_out, stride_ob, stride_oh};
+  const cudaError_t e = launch_paged_evict(c, p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? I4B_OK : fail_cuda(e);
+}
+
+int i4b_token_logprobs(const void* x, int dtype, int64_t rows, int64_t n, int64_t stride_x, const int64_t* targets,
+                       int64_t top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                       void* stream) {
+  if (dtype != I4B_BF16 && dtype != I4B_F16 && dtype != I4B_F32) return I4B_ERR_INVALID_ARG;
+  if (rows < 0 || rows > INT32_MAX || n <= 0 || n > INT32_MAX - 64 || stride_x < 0 || top < 0 || top > I4B_MAX_TOP ||
+      top > n)
+    return I4B_ERR_SHAPE;
+  if (rows == 0) return I4B_OK;
+  if (!x || !targets || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_ids))) return I4B_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == I4B_F32 ? 4 : 2) != 0) return I4B_ERR_LAYOUT;
+  DevInfo d;
+  if (int st = current_device_info(&d)) return st;
+  const cudaError_t e = launch_token_logprobs(x, dtype, rows, n, stride_x, targets, int(top), logprobs, entropy,
+                                              top_logprobs, top_ids, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? I4B_OK : fail_cuda(e);
+}
+
 size_t i4b_tile_w4_bytes(int64_t N, int64_t K, int group_size) { return tile_w4_bytes(N, K, group_size); }
 
 int i4b_tile_w4(const int32_t* qweight, int64_t N, int64_t stride_qk, const uint16_t* scales, const uint16_t* zeros,

@@ -165,4 +165,62 @@ int launch_decode_layers(const i4b_decode_model& m, int num_sms, int smem_optin,
 unsigned int read_dk_error(bool clear);
 void set_decode_trace(void* buf, size_t bytes);
 
+// paged.cu (serving over a paged key-value cache)
+struct PagedCache {  // strides in elements; the last dimension (head_dim) is contiguous
+  uint16_t* k;
+  uint16_t* v;
+  int64_t ks_page, ks_head, ks_token, vs_page, vs_head, vs_token;
+  const int32_t* table;
+  int64_t table_stride;
+  int seqs, capacity;  // rows of the table; positions that a row's pages hold
+  int num_pages, kv_heads, page_size, head_dim;
+  uint32_t ps_mul;     // n / page_size = umulhi(n, ps_mul) >> ps_shift for n < 2^31
+  int ps_shift;
+  bool f16;
+};
+struct PagedAttn {
+  const uint16_t* q;
+  int64_t sqb, sqh;
+  const int32_t* lens;
+  uint16_t* out;
+  int nq;
+  float scale;
+  float* weights;
+  int64_t swb, swh;
+};
+struct PagedAttnWorkspace {
+  float* partials;
+  float* logits;
+  int64_t logit_stride;
+  float* ml;
+};
+struct PagedEvict {
+  const float* weights;
+  int64_t swb, swh;
+  const int32_t* lens;
+  const int32_t* new_table;
+  int64_t new_stride;
+  int budget, recent, width;
+  int32_t* new_lens;
+  int32_t* kept;
+  float* weights_out;
+  int64_t sob, soh;
+};
+void paged_set_page_size(PagedCache* c, int page_size);
+// Bytes of the attention workspace; fills *w with its parts at `base` when w is not null.
+size_t paged_attn_workspace(int seqs, int nq, int head_dim, int capacity, bool weights, int sms, void* base,
+                            PagedAttnWorkspace* w);
+int64_t paged_attn_tiles(const PagedCache& c, int nq);  // at full length: has to fit 31 bits
+cudaError_t launch_paged_attn(const PagedCache& c, const PagedAttn& a, const PagedAttnWorkspace& w, int sms,
+                              cudaStream_t s);
+cudaError_t launch_paged_append(const PagedCache& c, const uint16_t* qkv, int64_t sqkv, int64_t tokens, const void* cosT,
+                                const void* sinT, bool table32, int max_pos, const int32_t* positions,
+                                const int32_t* slots, const int32_t* seqs, uint16_t* q_out, int nq, cudaStream_t s);
+cudaError_t launch_paged_evict(const PagedCache& c, const PagedEvict& e, cudaStream_t s);
+
+// logprobs.cu
+cudaError_t launch_token_logprobs(const void* x, int dtype, int64_t rows, int64_t n, int64_t stride,
+                                  const int64_t* targets, int top, float* logprobs, float* entropy, float* top_lp,
+                                  int64_t* top_ids, cudaStream_t s);
+
 }  // namespace i4b

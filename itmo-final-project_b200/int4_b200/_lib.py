@@ -5,6 +5,7 @@ if the library is missing, or the device is not a B200, every call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -47,6 +48,15 @@ _SIGNATURES = {
                                       ctypes.c_float, _c_vp]),
     "i4b_silu_mul": (_c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
     "i4b_argmax_rows": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_vp]),
+    "i4b_paged_kv_append": (_c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_int, _c_i64, _c_vp, _c_vp,
+                                     _c_vp, _c_vp, _c_vp]),
+    "i4b_paged_attention_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int]),
+    "i4b_paged_decode_attention": (_c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, ctypes.c_float, _c_vp, _c_vp,
+                                            _c_i64, _c_i64, _c_vp, _c_size, _c_vp]),
+    "i4b_paged_evict": (_c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64,
+                                 _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
+    "i4b_token_logprobs": (_c_int, [_c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp,
+                                    _c_vp]),
     "i4b_set_pdl": (None, [_c_int]),
     "i4b_set_w4_kernel_override": (None, [_c_int, _c_int, _c_int]),
     "i4b_set_w4_small_m_override": (None, [_c_int]),
@@ -81,6 +91,17 @@ class DecodeModel(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("tokens", "pos", "embed", "w_qkv", "w_o", "w_gu", "w_down", "ln1",
                                                "ln2", "cos_table", "sin_table", "k_cache", "v_cache", "h_out",
                                                "peers")]
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """``i4b_paged_cache`` of include/int4_b200.h."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("k_stride_page", "k_stride_head", "k_stride_token", "v_stride_page",
+                                              "v_stride_head", "v_stride_token")] + \
+               [("block_table", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("table_stride", "num_pages", "kv_heads", "page_size", "head_dim",
+                                              "seqs", "max_pages")] + [("dtype", ctypes.c_int32)]
 
 
 class Int4B200Error(RuntimeError):
@@ -124,6 +145,11 @@ def check(status: int, what: str) -> None:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (nothing to do, and nothing spent, where it is already)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 # Per (device, stream) workspace, zero-filled once; the kernels leave their

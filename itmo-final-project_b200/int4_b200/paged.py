@@ -1,0 +1,199 @@
+"""Serving over a paged key-value cache: sequences of different lengths, bounded memory.
+
+``decode`` runs a batch at one position over a static cache.  Here every sequence has its own length, and its keys and
+values lie in fixed-size pages that a block table names:
+
+* ``paged_kv_append``         rotary embedding of a step's (or a prompt's) tokens, keys and values into their pages;
+* ``paged_decode_attention``  one query token per sequence over its pages, grouped-query, split over the length and
+  joined; on request it adds up the attention weight that every cached slot receives;
+* ``paged_evict``             the slots of highest accumulated weight and the most recent ones, copied into new pages.
+
+The caches are views ``[pages, kv_heads, page_size, head_dim]`` of any strides that keep a row's ``head_dim`` values
+together (so ``[pages, page_size, kv_heads, head_dim]`` memory transposed will do), bf16 or fp16, head_dim 64 or 128,
+page_size a multiple of 8.  All indices and lengths are int32 tensors on the device: nothing here waits for the GPU,
+and every call can be captured in a CUDA graph.  The functions have no backward pass.  No counterpart in the
+reference, whose decode benchmark uses transformers' StaticCache (``benchmarks/eval_llama.py:121-183``).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _on_gpu(device: torch.device, *tensors) -> None:
+    """Every tensor on the one CUDA device."""
+    if device.type != "cuda":
+        raise ValueError("int4_b200 computes on the GPU only: the tensors must be CUDA tensors")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {t.device} and {device}: one call works on one device")
+
+
+def _indices(t: torch.Tensor, name: str, n: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} values")
+
+
+def _table(t: torch.Tensor, name: str) -> None:
+    if t.dtype != torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be an int32 tensor [sequences, pages] with unit stride along the pages")
+
+
+def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> _lib.PagedCacheStruct:
+    _need(k.dim() == 4 and k.shape == v.shape, "k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim]")
+    _need(k.dtype in _HALF and v.dtype == k.dtype, "k_cache and v_cache must both be bfloat16 or both float16")
+    _table(table, "block_table")
+    pages, heads, page, dim = k.shape
+    _need(dim in (64, 128), f"head_dim {dim}: 64 and 128 are supported")
+    _need(page > 0 and page % 8 == 0, f"page size {page}: a multiple of 8 is needed")
+    ks, vs = k.stride(), v.stride()
+    _need(ks[3] == 1 and vs[3] == 1, "the caches' last dimension must have unit stride")
+    seqs, width = table.shape
+    return _lib.PagedCacheStruct(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.data_ptr(),
+                                 table.stride(0), pages, heads, page, dim, seqs, width, _lib.DTYPE_CODE[k.dtype])
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy of it if not every row of the last dimension starts on a 16-byte boundary (2-byte elements)."""
+    s = t.stride()
+    if s[-1] == 1 and t.data_ptr() % 16 == 0 and all(x % 8 == 0 or n <= 1 for x, n in zip(s[:-1], t.shape)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def paged_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                    slots: torch.Tensor, block_table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
+                    seqs: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary embedding of the tokens ``qkv[T, (nq + 2 nkv) * head_dim]`` (q, k and v heads in that order); keys and
+    values go into the cache, the rotated queries ``[T, nq, head_dim]`` are returned.
+
+    Token i takes its angle from row ``positions[i]`` of ``cos`` / ``sin`` ``[max_pos, head_dim]`` (the cache's dtype
+    or float32) and goes to slot ``slots[i]`` of sequence ``seqs[i]`` (without ``seqs``: sequence i).  A slot or
+    sequence outside ``block_table``, or a page outside the cache, writes nothing (padding); a position outside the
+    tables gives a zero query and writes nothing.  Two tokens of a call must not name the same slot of a sequence."""
+    c = _cache(k_cache, v_cache, block_table)
+    nkv, dim = k_cache.shape[1], k_cache.shape[3]
+    _need(qkv.dim() == 2 and qkv.dtype == k_cache.dtype, "qkv must be [tokens, (nq + 2 nkv) * head_dim] of the caches' dtype")
+    T, width = qkv.shape
+    nq = width // dim - 2 * nkv
+    _need(width % dim == 0 and nq > 0, f"qkv rows of {width} values do not hold {nkv} key and value heads of {dim} and queries")
+    _need(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == dim and cos.shape[0] > 0
+          and cos.dtype == sin.dtype and cos.dtype in (k_cache.dtype, torch.float32) and cos.is_contiguous()
+          and sin.is_contiguous(), "cos and sin must be contiguous [max_pos, head_dim], of the caches' dtype or float32")
+    _indices(positions, "positions", T)
+    _indices(slots, "slots", T)
+    if seqs is not None:
+        _indices(seqs, "seqs", T)
+    else:
+        _need(T <= block_table.shape[0], f"{T} tokens without seqs, and a block table of {block_table.shape[0]} sequences")
+    if out is None:
+        out = torch.empty((T, nq, dim), dtype=qkv.dtype, device=qkv.device)
+    else:
+        _need(out.shape == (T, nq, dim) and out.dtype == qkv.dtype and out.is_contiguous(),
+              "out must be a contiguous [tokens, nq, head_dim] of the caches' dtype")
+    dev = qkv.device
+    _on_gpu(dev, k_cache, v_cache, block_table, cos, sin, positions, slots, seqs, out)
+    qkv = _rows16(qkv)
+    with _lib.on_device(dev):
+        st = _lib.lib().i4b_paged_kv_append(ctypes.byref(c), qkv.data_ptr(), qkv.stride(0), T, nq, cos.data_ptr(),
+                                            sin.data_ptr(), _lib.DTYPE_CODE[cos.dtype], cos.shape[0],
+                                            positions.data_ptr(), slots.data_ptr(),
+                                            None if seqs is None else seqs.data_ptr(), out.data_ptr(),
+                                            _lib.stream_handle(dev))
+    _lib.check(st, "paged_kv_append")
+    return out
+
+
+def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                           lens: torch.Tensor, *, scale: float | None = None, weights: torch.Tensor | None = None,
+                           out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one query token per sequence, ``q[B, nq, head_dim]``, over slots ``0..lens[b]-1`` of its pages;
+    query head h reads kv head ``h // (nq // nkv)``.  Returns ``[B, nq, head_dim]`` (zeros for an empty sequence).
+
+    ``scale`` is head_dim ** -0.5 unless given.  ``weights`` (float32 ``[B, nkv, >= pages * page_size]``) is added to
+    in place: slot j of a sequence gets its probability summed over the query heads of the kv head, which is what
+    ``paged_evict`` selects by.  Lengths are clamped to what the block table's rows can hold."""
+    c = _cache(k_cache, v_cache, block_table)
+    nkv, page, dim = k_cache.shape[1:]
+    B, width = block_table.shape
+    _need(q.dim() == 3 and q.shape[0] == B and q.shape[2] == dim and q.dtype == k_cache.dtype,
+          "q must be [sequences, nq, head_dim] of the caches' dtype")
+    nq = q.shape[1]
+    _need(nq > 0 and nq % nkv == 0, f"{nq} query heads do not divide over {nkv} kv heads")
+    _indices(lens, "lens", B)
+    if weights is not None:
+        _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
+              and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1),
+              f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
+    if out is None:
+        out = torch.empty((B, nq, dim), dtype=q.dtype, device=q.device)
+    else:
+        _need(out.shape == (B, nq, dim) and out.dtype == q.dtype and out.is_contiguous(),
+              "out must be a contiguous [sequences, nq, head_dim] of the caches' dtype")
+    dev = q.device
+    _on_gpu(dev, k_cache, v_cache, block_table, lens, weights, out)
+    q = _rows16(q)
+    L = _lib.lib()
+    with _lib.on_device(dev):
+        need = L.i4b_paged_attention_workspace_size(B, nq, nkv, dim, width * page, weights is not None)
+        # from torch's allocator each time: two captured graphs never share it, and eager streams do not either
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        st = L.i4b_paged_decode_attention(ctypes.byref(c), q.data_ptr(), q.stride(0), q.stride(1), nq, lens.data_ptr(),
+                                          dim ** -0.5 if scale is None else scale, out.data_ptr(),
+                                          None if weights is None else weights.data_ptr(),
+                                          0 if weights is None else weights.stride(0),
+                                          0 if weights is None else weights.stride(1), ws.data_ptr(), need,
+                                          _lib.stream_handle(dev))
+    _lib.check(st, "paged_decode_attention")
+    return out
+
+
+def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Tensor, k_cache: torch.Tensor,
+                v_cache: torch.Tensor, new_table: torch.Tensor, budget: int, *, recent: int = 0,
+                weights_out: torch.Tensor | None = None):
+    """Keep at most ``budget`` slots of every sequence and copy their keys and values, in order, into the pages of
+    ``new_table[B, >= ceil(budget / page_size)]``.
+
+    A sequence longer than the budget keeps, for each kv head by itself, its last ``recent`` slots and the
+    ``budget - recent`` of largest ``weights[B, nkv, W]`` among the others (ties: the lower slot); a shorter one keeps
+    all of them.  The new pages must not be pages that this call reads.  Returns ``(new_lens[B], kept[B, nkv, budget],
+    weights_out[B, nkv, W])``: the lengths afterwards, the slots kept (-1 behind the last one) and their weights (zeros
+    behind the last; ``weights_out`` may be ``weights`` itself)."""
+    c = _cache(k_cache, v_cache, block_table)
+    nkv, page = k_cache.shape[1:3]
+    B, width = block_table.shape
+    _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
+          and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1),
+          f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
+    _indices(lens, "lens", B)
+    _table(new_table, "new_table")
+    _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget} and recent {recent}: 0 <= recent <= budget, budget >= 1")
+    _need(new_table.shape[0] == B and new_table.shape[1] * page >= budget,
+          f"new_table must hold {-(-budget // page)} pages for each of {B} sequences")
+    dev = weights.device
+    if weights_out is None:
+        weights_out = torch.empty(weights.shape, dtype=torch.float32, device=dev)
+    else:
+        _need(weights_out.shape == weights.shape and weights_out.dtype == torch.float32
+              and (weights.shape[2] <= 1 or weights_out.stride(2) == 1), "weights_out must be float32 of the weights' shape")
+    _on_gpu(dev, k_cache, v_cache, block_table, lens, new_table, weights_out)
+    new_lens = torch.empty(B, dtype=torch.int32, device=dev)
+    kept = torch.empty((B, nkv, budget), dtype=torch.int32, device=dev)
+    with _lib.on_device(dev):
+        st = _lib.lib().i4b_paged_evict(ctypes.byref(c), weights.data_ptr(), weights.stride(0), weights.stride(1),
+                                        weights.shape[2], lens.data_ptr(), new_table.data_ptr(), new_table.stride(0),
+                                        new_table.shape[1], budget, recent, new_lens.data_ptr(), kept.data_ptr(),
+                                        weights_out.data_ptr(), weights_out.stride(0), weights_out.stride(1),
+                                        _lib.stream_handle(dev))
+    _lib.check(st, "paged_evict")
+    return new_lens, kept, weights_out
