@@ -42,6 +42,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {  // round to nea
   }
 }
 
+// The transpose of an 8 x 8 matrix of 16-bit values held two to a lane (row lane / 4, columns 2 (lane % 4) and + 1).
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // n / page_size for n < 2^31, by multiplication (page sizes need not be powers of two).
 __device__ __forceinline__ int page_of(const PagedCache& c, int n) {
   return int(__umulhi(uint32_t(n), c.ps_mul) >> c.ps_shift);
@@ -139,22 +146,30 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedCache c, c
 
 // ------------------------------------------------------------------ attention
 
-// The cached positions of every (sequence, kv head, tile of 16 query heads) item are cut into tiles of 32; the
-// items' tiles, one item behind the other, are dealt in equal consecutive runs to the grid's warps, each of which
-// works by itself.  A run that holds an item whole writes its output; the pieces of an item that several runs share
-// go to the workspace as (max, sum, unnormalised output) and paged_attn_join adds them in the runs' order.  The deal
-// depends on the lengths alone, so results repeat bit by bit.
+// The cached positions of every (sequence, kv head, 16 query heads) item are cut into tiles; the items' tiles, one item
+// behind the other, are dealt in equal consecutive runs to the grid's warps, each of which works by itself.  A run that
+// holds an item whole writes its output; the pieces of an item that several runs share go to the workspace as (max,
+// sum, unnormalised output) and paged_attn_join adds them in the runs' order.  The deal depends on the lengths alone,
+// so results repeat bit by bit.
+//
+// Both products are taken with the positions (or the head's dims) as the rows of the matrix instruction and the query
+// heads as its 8 columns -- S^T = K Q^T, O^T = V^T P^T -- so that a group of 4 or 8 query heads fills half or all of
+// it, not a quarter or half of 16 rows.  Between them P^T goes through an 8 x 8 transposition of registers.
+//
+// Bound by the bytes of K and V: the products are a few percent of what even mma.sync can do, so what counts is bytes
+// in flight and whole 128-byte lines for each quarter of a warp.  Each warp keeps three units of 4 KB (a tile's keys or
+// its values) on their way, as a queue of its own in shared memory: a quarter copies one row (or half of a 256-byte
+// one), and the 16-byte words are placed so that neither that nor the reading of the MMA fragments meets a bank twice.
+// (With every lane copying just the words of its own fragments, which needs no exchange, the values came in 32-byte
+// pieces: 160 us against 129 for 687 MB.)
 constexpr int kAttnWarps = 4;
-constexpr int kAttnCtasPerSm = 2;
-constexpr int kTile = 32;
-constexpr int kMinTiles = 2;  // per warp: below this the join costs more than the split saves
+constexpr int kUnit = 4096;  // bytes of a tile's keys, or values
+constexpr int kUnits = 3;    // in flight per warp
+constexpr int kMinTiles = 2;
 
-// Tiles of sequence b before / in it, from the lengths; shared by the attention kernel and its join.
-struct Deal {
-  int H;      // items per sequence: kv heads x tiles of query heads
-  int total;  // tiles of all items
-  int per;    // tiles of a run
-};
+__host__ __device__ constexpr int attn_ctas(int head_dim, bool two) { return two && head_dim == 128 ? 3 : 4; }  // per SM
+
+__host__ __device__ constexpr int tile_of(int head_dim) { return kUnit / 2 / head_dim; }  // 32 or 16 positions
 
 __device__ __forceinline__ int clamped_len(const PagedCache& c, const int32_t* lens, int b) {
   const int n = __ldg(lens + b);
@@ -166,27 +181,28 @@ __device__ __forceinline__ int run_tiles(int total, int workers) {
   return per < kMinTiles ? kMinTiles : per;
 }
 
-struct Cursor {
-  int b, h, tile, nt, len;
-};
-
 template <bool F16, int HD, bool TWO, bool WEIGHTS>
-__global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtasPerSm)
+__global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
     paged_attn_kernel(const PagedCache c, const uint16_t* __restrict__ q, int64_t sqb, int64_t sqh,
                       const int32_t* __restrict__ lens, uint16_t* __restrict__ out, int nq, int HT, float scale_log2,
                       float* __restrict__ partials, float* __restrict__ logits, int64_t logit_stride,
                       float* __restrict__ ml) {
-  constexpr int HC = HD / 32;              // 16-byte chunks of a key row that a lane owns
-  constexpr int VC = HD / 64;              // 16-byte chunks of a value row that a lane owns
-  constexpr int kHalf = kTile * HD * 2;    // bytes of a tile's keys (or values)
-  constexpr int NB = 24576 / kHalf;        // halves in flight per warp
-  constexpr int R = TWO ? 2 : 1;           // rows of 8 query heads
+  constexpr int KT = tile_of(HD);         // positions of a tile
+  constexpr int KI = KT / 16, KR = KT / 8; // blocks of 16 positions; key rows that a lane owns
+  constexpr int HC = HD / 32;              // 16-byte chunks of a key row that a lane uses: t + 4h
+  constexpr int VC = HD / 64;              // 16-byte chunks of a value row that a lane uses: g + 8v
+  constexpr int R = TWO ? 2 : 1;           // blocks of 8 query heads
+  static_assert(KR <= 4, "a lane's 2 KR value rows lie in one page: pages are multiples of 8");
+  // Row r of block i is position KR * (r % 8) + KI * (r / 8) + i of the tile: lane (g, t) uses the KR consecutive key
+  // rows from KR * g (rows g and g + 8 of every block) and the 2 KR value rows from 2 KR * t (k = 2t, 2t + 1, 2t + 8,
+  // 2t + 9 of every block).  Key word (row j, chunk t + 4h) of lane (g, t) lies at 32 (HC j + h) + ((4g + t) ^ 4 (h & 1)),
+  // value word (row j, chunk g + 8v) at 32 (VC j + v) + 8t + (g ^ 2t).
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int scan_tmp[kAttnWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint4* ring = reinterpret_cast<uint4*>(smem) + warp * (NB * kHalf / 16);
-  int* pre = reinterpret_cast<int*>(smem + kAttnWarps * NB * kHalf);  // [B + 1] first tile of each sequence
-  int* len = pre + c.seqs + 1;                                       // [B]
+  uint4* ring = reinterpret_cast<uint4*>(smem + warp * (kUnits * kUnit));
+  int* pre = reinterpret_cast<int*>(smem + kAttnWarps * kUnits * kUnit);  // [B + 1] first tile of each sequence
+  int* len = pre + c.seqs + 1;                                            // [B]
   const int H = c.kv_heads * HT, B = c.seqs, G = nq / c.kv_heads;
 
   // exclusive scan of the sequences' tiles
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtasPerSm)
     for (int b0 = 0; b0 < B; b0 += kAttnWarps * 32) {
       const int b = b0 + tid;
       const int L = b < B ? clamped_len(c, lens, b) : 0;
-      int v = (L + kTile - 1) / kTile * H;
+      int v = (L + KT - 1) / KT * H;
       const int own = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -227,263 +243,349 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtasPerSm)
   if (begin64 >= total) return;
   const int begin = int(begin64), ntiles = min(per, total - begin);
 
-  Cursor cc;  // what is computed
+  struct Item {
+    int b, h, len, nt;  // sequence; kv head and tile of query heads; the sequence's length and tiles
+  };
+  Item ci;     // the item being computed, and its tile
+  int ctile;
   {
     int lo = 0, hi = B;  // pre[lo] <= begin < pre[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (pre[mid] <= begin) lo = mid; else hi = mid;
     }
-    cc.b = lo;
-    cc.len = len[lo];
-    cc.nt = (cc.len + kTile - 1) / kTile;
+    ci.b = lo;
+    ci.len = len[lo];
+    ci.nt = (ci.len + KT - 1) / KT;
     const int off = begin - pre[lo];
-    cc.h = off / cc.nt;
-    cc.tile = off - cc.h * cc.nt;
+    ci.h = off / ci.nt;
+    ctile = off - ci.h * ci.nt;
   }
-  auto advance = [&](Cursor& x) {
-    if (++x.tile < x.nt) return;
-    x.tile = 0;
+  auto next_item = [&](Item& x) {
     if (++x.h < H) return;
     x.h = 0;
     do ++x.b;
     while (x.b < B && len[x.b] == 0);
     if (x.b < B) {
       x.len = len[x.b];
-      x.nt = (x.len + kTile - 1) / kTile;
+      x.nt = (x.len + KT - 1) / KT;
     }
   };
 
-  // ---- loads: lane (g, t) copies for itself the keys 4g..4g+3, chunks t + 4h, and the values of positions
-  // 8t..8t+7, chunks g + 8c: exactly the words its MMA fragments need, so no lane waits for another.
-  Cursor ic = cc;  // what is requested
-  int iu = 0, islot = 0;
-  int kp = -1, vp = -1, krow = 0, vrow = 0;
-  uint32_t vok = 0;  // bit n % 32: whether tile n's value page is there
+  // ---- requests.  Tile x's keys are requested after the values of tile x - 2 have been used, its values after the
+  // keys of tile x - 1; its page numbers are read half a tile before that.
+  Item ri = ci;    // the item being requested, its tile, and what is the same for all its tiles
+  int rtile = ctile;
+  const int32_t* rtable;
+  const uint16_t *rk, *rv;
+  auto enter = [&]() {
+    const int kvh = HT == 1 ? ri.h : ri.h / HT;
+    rtable = c.table + int64_t(ri.b) * c.table_stride;
+    rk = c.k + kvh * c.ks_head + 8 * (lane & 7);
+    rv = c.v + kvh * c.vs_head + 8 * (lane & 7);
+  };
+  enter();
+  // this lane copies chunk lane % 8 (+ 8y) of the key rows from KR * (4x + lane / 8), x = 0, 1, and of the value rows
+  // from 2 KR * (lane / 8)
+  const int lq = lane >> 3, l8 = lane & 7;
+  const int kdst = 32 * (l8 >> 2) + ((4 * lq + (l8 & 3)) ^ (4 * (l8 >> 2))), vdst = 8 * lq + (l8 ^ (2 * lq));
+  int requested = 0;   // tiles whose keys were requested
+  int kpage[2], krow[2], vpage = -1, vrow = 0;
+  krow[0] = krow[1] = 0;
   auto fetch_pages = [&]() {
-    const int32_t* trow = c.table + int64_t(ic.b) * c.table_stride;
-    const int kpos = ic.tile * kTile + 4 * g, vpos = ic.tile * kTile + 8 * t;
-    kp = vp = -1;
-    if (kpos < ic.len) {
-      const int pi = page_of(c, kpos);
-      krow = kpos - pi * c.page_size;
-      kp = page_entry(c, trow, pi);
-    }
-    if (vpos < ic.len) {
+    kpage[0] = kpage[1] = vpage = -1;
+    if (requested >= ntiles) return;
+    const int vpos = rtile * KT + 2 * KR * lq;
+    if (vpos < ri.len) {
       const int pi = page_of(c, vpos);
       vrow = vpos - pi * c.page_size;
-      vp = page_entry(c, trow, pi);
+      vpage = __ldg(rtable + pi);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int kpos = rtile * KT + KR * (4 * x + lq);
+      if (kpos < ri.len) {
+        const int pi = page_of(c, kpos);
+        krow[x] = kpos - pi * c.page_size;
+        kpage[x] = __ldg(rtable + pi);
+      }
     }
   };
-  auto issue = [&]() {
-    if (iu < 2 * ntiles) {
-      uint4* dst = ring + islot * (kHalf / 16) + lane;
-      const int kvh = HT == 1 ? ic.h : ic.h / HT;
-      if ((iu & 1) == 0) {
-        const int left = ic.len - (ic.tile * kTile + 4 * g);
-        const uint16_t* src = c.k + int64_t(kp) * c.ks_page + int64_t(kvh) * c.ks_head + int64_t(krow) * c.ks_token + 8 * t;
+  const uint16_t* vsrc = nullptr;  // the first of the value rows of the tile whose values are requested next
+  int vleft = 0;                   // how many of them exist
+  uint32_t flags = 0;  // two bits for each of the last tiles (x & 7): every position there; this lane's key page there
+  auto request_keys = [&](uint4* dst) {
+    __syncwarp();  // the slot has been read by every lane
+    if (requested < ntiles) {
+      const bool ok0 = uint32_t(kpage[0]) < uint32_t(c.num_pages), ok1 = uint32_t(kpage[1]) < uint32_t(c.num_pages);
+      const bool vok = uint32_t(vpage) < uint32_t(c.num_pages);
+      const uint32_t b0 = __ballot_sync(0xFFFFFFFFu, ok0), b1 = __ballot_sync(0xFFFFFFFFu, ok1);
+      const bool full = (rtile + 1) * KT <= ri.len && (b0 & b1) == 0xFFFFFFFFu;  // (a tile's values have its keys' pages)
+      const uint32_t f = (full ? 1u : 0u) | ((g & 4 ? b1 : b0) >> (8 * (g & 3)) & 1u) << 1;
+      const int sh = (requested & 7) * 2;
+      flags = (flags & ~(3u << sh)) | (f << sh);
+      vsrc = rv + vpage * c.vs_page + vrow * c.vs_token;
+      vleft = vok ? ri.len - (rtile * KT + 2 * KR * lq) : 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool ok = kp >= 0 && j < left;
+      for (int x = 0; x < 2; ++x) {
+        const uint16_t* src = rk + kpage[x] * c.ks_page + krow[x] * c.ks_token;
+        const int left = (x ? ok1 : ok0) ? ri.len - (rtile * KT + KR * (4 * x + lq)) : 0;
 #pragma unroll
-          for (int h = 0; h < HC; ++h)
-            cp_async_16(dst + (j * HC + h) * 32, ok ? src + j * c.ks_token + 32 * h : c.k, ok ? 16u : 0u);
-        }
-      } else {
-        const int left = ic.len - (ic.tile * kTile + 8 * t);
-        const uint16_t* src = c.v + int64_t(vp) * c.vs_page + int64_t(kvh) * c.vs_head + int64_t(vrow) * c.vs_token + 8 * g;
+        for (int j = 0; j < KR; ++j, src += c.ks_token)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool ok = vp >= 0 && j < left;  // rows behind the end arrive as zeros, whatever they hold
-#pragma unroll
-          for (int v = 0; v < VC; ++v)
-            cp_async_16(dst + (j * VC + v) * 32, ok ? src + j * c.vs_token + 64 * v : c.v, ok ? 16u : 0u);
-        }
-        const uint32_t bit = 1u << ((iu >> 1) & 31);
-        vok = vp >= 0 ? (vok | bit) : (vok & ~bit);
-        if (iu + 1 < 2 * ntiles) {
-          advance(ic);
-          fetch_pages();
-        }
+          for (int y = 0; y < HC / 2; ++y) {
+            uint4* to = dst + 32 * (HC * j + 2 * y) + (kdst ^ (16 * x));
+            if (full)
+              cp_async_16(to, src + 64 * y, 16u);
+            else
+              cp_async_16(to, j < left ? src + 64 * y : c.k, j < left ? 16u : 0u);
+          }
+      }
+      ++requested;
+      if (++rtile == ri.nt) {
+        rtile = 0;
+        next_item(ri);
+        if (requested < ntiles) enter();
       }
     }
     cp_async_commit();
-    ++iu;
-    islot = islot + 1 == NB ? 0 : islot + 1;
   };
-  fetch_pages();
+  auto request_values = [&](uint4* dst, int x) {  // of tile x
+    __syncwarp();
+    if (x < ntiles) {
+      const bool full = flags >> ((x & 7) * 2) & 1u;
+      const uint16_t* src = vsrc;
 #pragma unroll
-  for (int i = 0; i < NB; ++i) issue();
+      for (int j = 0; j < 2 * KR; ++j, src += c.vs_token)
+#pragma unroll
+        for (int v = 0; v < VC; ++v) {
+          uint4* to = dst + 32 * (VC * j + v) + vdst;
+          if (full)
+            cp_async_16(to, src + 64 * v, 16u);
+          else
+            cp_async_16(to, j < vleft ? src + 64 * v : c.v, j < vleft ? 16u : 0u);  // rows that do not exist: zeros
+        }
+    }
+    cp_async_commit();
+  };
+  constexpr int kSlot = kUnit / 16;
+  fetch_pages();
+  request_keys(ring);
+  request_values(ring + kSlot, 0);
+  fetch_pages();
+  request_keys(ring + 2 * kSlot);
 
-  uint32_t qa[2 * HC][4];
-  float o[8 * VC][4], m[R], l[R];
-  int cslot = 0, seg_first = 0, seg_tile0 = cc.tile;
+  // A negative scale turns the queries' signs instead, so that the largest product has the largest score.
+  const uint32_t flip = scale_log2 < 0.0f ? 0x80008000u : 0u;
+  const float scl = fabsf(scale_log2);
+  uint32_t qb[R][2 * HC][2];
+  float o[R][4 * VC][4], m[R][2], l[R][2];  // of heads 2t and 2t + 1 of each block of 8
+  int slot = 0, seg_first = 0, seg_tile0 = ctile;
   bool fresh = true;
   for (int n = 0; n < ntiles; ++n) {
-    const int kvh = HT == 1 ? cc.h : cc.h / HT;
-    const int head0 = kvh * G + (HT == 1 ? 0 : cc.h % HT) * 16;
-    const int rows = min(16, kvh * G + G - head0);  // query heads of this item
     if (fresh) {
       fresh = false;
-      const uint16_t* qr = q + int64_t(cc.b) * sqb + int64_t(head0) * sqh + 8 * t;
-#pragma unroll
-      for (int h = 0; h < HC; ++h) {
-        uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
-        if (g < rows) a = __ldg(reinterpret_cast<const uint4*>(qr + int64_t(g) * sqh + 32 * h));
-        if (TWO && g + 8 < rows) b = __ldg(reinterpret_cast<const uint4*>(qr + int64_t(g + 8) * sqh + 32 * h));
-        qa[2 * h][0] = a.x, qa[2 * h][2] = a.y, qa[2 * h + 1][0] = a.z, qa[2 * h + 1][2] = a.w;
-        qa[2 * h][1] = b.x, qa[2 * h][3] = b.y, qa[2 * h + 1][1] = b.z, qa[2 * h + 1][3] = b.w;
-      }
-#pragma unroll
-      for (int i = 0; i < 8 * VC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-#pragma unroll
-      for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.0f;
-    }
-    // ---- scores: column n of block j is position 4n + j of the tile (as the keys were loaded)
-    cp_async_wait<NB - 1>();
-    float s[4][4];
-    {
-      const uint4* src = ring + cslot * (kHalf / 16) + lane;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int h = 0; h < HC; ++h) {
-          const uint4 kf = src[(j * HC + h) * 32];
-          if (h == 0)
-            mma_16816_first<F16>(s[j], qa[0], kf.x, kf.y);
-          else
-            mma_16816<F16>(s[j], qa[2 * h], kf.x, kf.y);
-          mma_16816<F16>(s[j], qa[2 * h + 1], kf.z, kf.w);
-        }
-      }
-    }
-    cslot = cslot + 1 == NB ? 0 : cslot + 1;
-    issue();
-    // ---- softmax over this tile; the lane's columns are positions 8t + j and 8t + 4 + j
-    const int left = (vok >> (n & 31)) & 1u ? cc.len - (cc.tile * kTile + 8 * t) : 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        s[j][2 * r] = j < left ? s[j][2 * r] * scale_log2 : -INFINITY;
-        s[j][2 * r + 1] = 4 + j < left ? s[j][2 * r + 1] * scale_log2 : -INFINITY;
-      }
-    if constexpr (WEIGHTS) {
+      const int kvh = HT == 1 ? ci.h : ci.h / HT, head0 = kvh * G + (HT == 1 ? 0 : ci.h % HT) * 16;
+      const int rows = min(16, kvh * G + G - head0);  // query heads of this item
+      const uint16_t* qr = q + int64_t(ci.b) * sqb + int64_t(head0) * sqh + 8 * t;
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (g + 8 * r < rows) {
-          float4* dst = reinterpret_cast<float4*>(logits + (int64_t(cc.b) * nq + head0 + g + 8 * r) * logit_stride +
-                                                  cc.tile * kTile + 8 * t);
-          dst[0] = make_float4(s[0][2 * r], s[1][2 * r], s[2][2 * r], s[3][2 * r]);
-          dst[1] = make_float4(s[0][2 * r + 1], s[1][2 * r + 1], s[2][2 * r + 1], s[3][2 * r + 1]);
+#pragma unroll
+        for (int h = 0; h < HC; ++h) {
+          uint4 a = make_uint4(0u, 0u, 0u, 0u);
+          if (g + 8 * r < rows) a = __ldg(reinterpret_cast<const uint4*>(qr + int64_t(g + 8 * r) * sqh + 32 * h));
+          qb[r][2 * h][0] = a.x ^ flip, qb[r][2 * h][1] = a.y ^ flip;
+          qb[r][2 * h + 1][0] = a.z ^ flip, qb[r][2 * h + 1][1] = a.w ^ flip;
         }
-    }
-    bool grew = false;
-    float mn[R], base[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float mx = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
-#pragma unroll
-      for (int j = 1; j < 4; ++j) mx = fmaxf(mx, fmaxf(s[j][2 * r], s[j][2 * r + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-      mn[r] = fmaxf(m[r], mx);
-      grew |= mn[r] > m[r];
-      base[r] = mn[r] == -INFINITY ? 0.0f : mn[r];  // nothing seen yet: every probability is exp2(-inf) = 0
-    }
-    if (__any_sync(0xFFFFFFFFu, grew)) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float f = ex2(m[r] - base[r]);  // m = -inf gives 0
-        l[r] *= f;
-        m[r] = mn[r];
 #pragma unroll
-        for (int i = 0; i < 8 * VC; ++i) o[i][2 * r] *= f, o[i][2 * r + 1] *= f;
+        for (int i = 0; i < 4 * VC; ++i) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.0f;
+        m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
       }
+    }
+    // ---- scores
+    cp_async_wait<kUnits - 1>();
+    __syncwarp();
+    float s[R][KI][4];  // rows g, g, g + 8, g + 8 of block i; heads 2t, 2t + 1, 2t, 2t + 1
+    {
+      const uint4* src = ring + slot * kSlot;
+#pragma unroll
+      for (int i = 0; i < KI; ++i)
+#pragma unroll
+        for (int h = 0; h < HC; ++h) {
+          const uint4 x = src[(i * HC + h) * 32 + (lane ^ (4 * (h & 1)))], y = src[((KI + i) * HC + h) * 32 + (lane ^ (4 * (h & 1)))];
+          const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            if (h == 0)
+              mma_16816_first<F16>(s[r][i], a0, qb[r][0][0], qb[r][0][1]);
+            else
+              mma_16816<F16>(s[r][i], a0, qb[r][2 * h][0], qb[r][2 * h][1]);
+            mma_16816<F16>(s[r][i], a1, qb[r][2 * h + 1][0], qb[r][2 * h + 1][1]);
+          }
+        }
+    }
+    request_values(ring + slot * kSlot, n + 1);
+    slot = slot == kUnits - 1 ? 0 : slot + 1;
+    fetch_pages();
+    // ---- softmax; the lane's scores are those of its key rows KR * g + KI * e + i, entries [i][2 * e + head]
+    const uint32_t f = flags >> ((n & 7) * 2);
+    if (!(f & 1u)) {
+      const int left = f >> 1 & 1u ? ci.len - (ctile * KT + KR * g) : 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < KI; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (KI * e + i >= left) s[r][i][2 * e] = s[r][i][2 * e + 1] = -INFINITY;
+    }
+    // The reference point m of the exponentials follows the maximum with a slack of 2^8: it moves, and what is summed
+    // so far is scaled, only when a score passes it by more (and with a head's first score).
+    bool grew = false;
+    float mx[R][2];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        mx[r][u] = fmaxf(s[r][0][u], s[r][0][2 + u]);
+#pragma unroll
+        for (int i = 1; i < KI; ++i) mx[r][u] = fmaxf(mx[r][u], fmaxf(s[r][i][u], s[r][i][2 + u]));
+        grew |= fmaf(mx[r][u], scl, -8.0f) > m[r][u];
+      }
+    if (__any_sync(0xFFFFFFFFu, grew)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float v = mx[r][u];
+          v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
+          v = fmaxf(m[r][u], v == -INFINITY ? v : v * scl);
+          const float k = v == -INFINITY ? 1.0f : ex2(m[r][u] - v);  // 0 for a head's first score
+          m[r][u] = v;
+          l[r][u] *= k;
+#pragma unroll
+          for (int i = 0; i < 4 * VC; ++i) o[r][i][u] *= k, o[r][i][2 + u] *= k;
+        }
+    }
+    if constexpr (WEIGHTS) {
+      const int kvh = HT == 1 ? ci.h : ci.h / HT, head0 = kvh * G + (HT == 1 ? 0 : ci.h % HT) * 16;
+      const int rows = min(16, kvh * G + G - head0);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (2 * t + u + 8 * r < rows) {
+            float* dst = logits + (int64_t(ci.b) * nq + head0 + 2 * t + u + 8 * r) * logit_stride + ctile * KT + KR * g;
+            float w[KR];
+#pragma unroll
+            for (int i = 0; i < KR; ++i) {
+              const float x = s[r][i % KI][2 * (i / KI) + u];
+              w[i] = x == -INFINITY ? x : x * scl;
+            }
+            if constexpr (KR == 2) {
+              *reinterpret_cast<float2*>(dst) = make_float2(w[0], w[1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < KR; i += 4)
+                *reinterpret_cast<float4*>(dst + i) = make_float4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+            }
+          }
     }
     // probabilities; rounded to the values' type for the second product (half a step each, as the output is),
     // summed unrounded
-    uint32_t pa[2][4];
+    uint32_t pb[R][KI][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int r = 0; r < R; ++r) {
+      const float n0 = m[r][0] == -INFINITY ? 0.0f : -m[r][0], n1 = m[r][1] == -INFINITY ? 0.0f : -m[r][1];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        uint32_t w = 0u;
-        if (r < R) {
-          const float p0 = ex2(s[j][2 * r] - base[r]), p1 = ex2(s[j][2 * r + 1] - base[r]);
-          l[r] += p0 + p1;
-          w = pack2<F16>(p0, p1);
+      for (int i = 0; i < KI; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x0 = s[r][i][2 * e], x1 = s[r][i][2 * e + 1];
+          float p0 = ex2(fmaf(x0, scl, n0)), p1 = ex2(fmaf(x1, scl, n1));
+          if (!(f & 1u)) {  // (a scale of 0 would make a NaN of a place that is not there)
+            p0 = x0 == -INFINITY ? 0.0f : p0;
+            p1 = x1 == -INFINITY ? 0.0f : p1;
+          }
+          l[r][0] += p0, l[r][1] += p1;
+          pb[r][i][e] = transpose8(pack2<F16>(p0, p1));
         }
-        pa[j >> 1][2 * (j & 1) + r] = w;
-      }
-    // ---- output: the pair (8t + j, 8t + 4 + j) of value rows meets the pair of probabilities of block j
-    cp_async_wait<NB - 1>();
+    }
+    // ---- output: dims 8(g + 8v) + 2w and + 2w + 1 are rows g and g + 8 of block 4v + w
+    cp_async_wait<kUnits - 1>();
+    __syncwarp();
     {
-      const uint4* src = ring + cslot * (kHalf / 16) + lane;
+      const uint4* src = ring + slot * kSlot + 8 * t + (g ^ (2 * t));
 #pragma unroll
       for (int v = 0; v < VC; ++v)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint4 a0 = src[((2 * k) * VC + v) * 32], b0 = src[((2 * k + 4) * VC + v) * 32];
-          const uint4 a1 = src[((2 * k + 1) * VC + v) * 32], b1 = src[((2 * k + 5) * VC + v) * 32];
-          const uint32_t x0[4] = {a0.x, a0.y, a0.z, a0.w}, y0[4] = {b0.x, b0.y, b0.z, b0.w};
-          const uint32_t x1[4] = {a1.x, a1.y, a1.z, a1.w}, y1[4] = {b1.x, b1.y, b1.z, b1.w};
+        for (int i = 0; i < KI; ++i) {
+          const uint4 a = src[(i * VC + v) * 32], b = src[((KR + i) * VC + v) * 32];
+          const uint4 d = src[((KI + i) * VC + v) * 32], e = src[((KR + KI + i) * VC + v) * 32];
+          const uint32_t x0[4] = {a.x, a.y, a.z, a.w}, y0[4] = {b.x, b.y, b.z, b.w};
+          const uint32_t x1[4] = {d.x, d.y, d.z, d.w}, y1[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            mma_16816<F16>(o[8 * v + 2 * w], pa[k], __byte_perm(x0[w], y0[w], 0x5410), __byte_perm(x1[w], y1[w], 0x5410));
-            mma_16816<F16>(o[8 * v + 2 * w + 1], pa[k], __byte_perm(x0[w], y0[w], 0x7632), __byte_perm(x1[w], y1[w], 0x7632));
+            const uint32_t va[4] = {__byte_perm(x0[w], y0[w], 0x5410), __byte_perm(x0[w], y0[w], 0x7632),
+                                    __byte_perm(x1[w], y1[w], 0x5410), __byte_perm(x1[w], y1[w], 0x7632)};
+#pragma unroll
+            for (int r = 0; r < R; ++r) mma_16816<F16>(o[r][4 * v + w], va, pb[r][i][0], pb[r][i][1]);
           }
         }
     }
-    cslot = cslot + 1 == NB ? 0 : cslot + 1;
-    issue();
+    request_keys(ring + slot * kSlot);
+    slot = slot == kUnits - 1 ? 0 : slot + 1;
     // ---- end of the item, or of this run
-    if (cc.tile == cc.nt - 1 || n == ntiles - 1) {
-      const bool whole = seg_tile0 == 0 && cc.tile == cc.nt - 1;
+    if (ctile == ci.nt - 1 || n == ntiles - 1) {
+      const int kvh = HT == 1 ? ci.h : ci.h / HT, head0 = kvh * G + (HT == 1 ? 0 : ci.h % HT) * 16;
+      const int rows = min(16, kvh * G + G - head0);
+      const bool whole = seg_tile0 == 0 && ctile == ci.nt - 1;
       float* part = partials + int64_t(2 * worker + (seg_first == 0 ? 0 : 1)) * (16 * (HD + 2));
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float ls = l[r] + __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
-        ls += __shfl_xor_sync(0xFFFFFFFFu, ls, 2);
-        if (g + 8 * r < rows) {
-          if (whole) {
-            const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;  // no position: zeros (a NaN stays one)
-            uint16_t* dst = out + (int64_t(cc.b) * nq + head0 + g + 8 * r) * HD;
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int v = 0; v < VC; ++v)
+        for (int u = 0; u < 2; ++u) {
+          float ls = l[r][u] + __shfl_xor_sync(0xFFFFFFFFu, l[r][u], 4);
+          ls += __shfl_xor_sync(0xFFFFFFFFu, ls, 8);
+          ls += __shfl_xor_sync(0xFFFFFFFFu, ls, 16);
+          const int row = 2 * t + u + 8 * r;
+          if (row < rows) {
+            if (whole) {
+              const float inv = ls > 0.0f || ls != ls ? 1.0f / ls : 0.0f;  // no position: zeros (a NaN stays one)
+              uint16_t* dst = out + (int64_t(ci.b) * nq + head0 + row) * HD;
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
+              for (int v = 0; v < VC; ++v) {
                 uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  w[i] = pack2<F16>(o[8 * v + 2 * i][2 * r + e] * inv, o[8 * v + 2 * i + 1][2 * r + e] * inv);
-                *reinterpret_cast<uint4*>(dst + 8 * (2 * t + e + 8 * v)) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int i = 0; i < 4; ++i) w[i] = pack2<F16>(o[r][4 * v + i][u] * inv, o[r][4 * v + i][2 + u] * inv);
+                *reinterpret_cast<uint4*>(dst + 8 * (g + 8 * v)) = make_uint4(w[0], w[1], w[2], w[3]);
               }
-            if (WEIGHTS && t == 0)
-              *reinterpret_cast<float2*>(ml + 2 * (int64_t(cc.b) * nq + head0 + g + 8 * r)) = make_float2(m[r], inv);
-          } else {
-            float* dst = part + (g + 8 * r) * HD;
+              if (WEIGHTS && g == 0)
+                *reinterpret_cast<float2*>(ml + 2 * (int64_t(ci.b) * nq + head0 + row)) = make_float2(m[r][u], inv);
+            } else {
+              float* dst = part + row * HD;
 #pragma unroll
-            for (int v = 0; v < VC; ++v)
+              for (int v = 0; v < VC; ++v)
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                  *reinterpret_cast<float4*>(dst + 8 * (2 * t + e + 8 * v) + 4 * i) =
-                      make_float4(o[8 * v + 4 * i][2 * r + e], o[8 * v + 4 * i + 1][2 * r + e],
-                                  o[8 * v + 4 * i + 2][2 * r + e], o[8 * v + 4 * i + 3][2 * r + e]);
-            if (t == 0) {
-              part[16 * HD + 2 * (g + 8 * r)] = m[r];
-              part[16 * HD + 2 * (g + 8 * r) + 1] = ls;
+                for (int i = 0; i < 4; i += 2)
+                  *reinterpret_cast<float4*>(dst + 8 * (g + 8 * v) + 2 * i) =
+                      make_float4(o[r][4 * v + i][u], o[r][4 * v + i][2 + u], o[r][4 * v + i + 1][u], o[r][4 * v + i + 1][2 + u]);
+              if (g == 0) *reinterpret_cast<float2*>(part + 16 * HD + 2 * row) = make_float2(m[r][u], ls);
             }
           }
         }
-      }
       fresh = true;
       seg_first = n + 1;
       seg_tile0 = 0;
     }
-    advance(cc);
+    if (++ctile == ci.nt) {
+      ctile = 0;
+      next_item(ci);
+    }
   }
   cp_async_wait<0>();
 }
@@ -495,17 +597,17 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const PagedCache c
                                                               uint16_t* __restrict__ out, int nq, int HT, int workers,
                                                               const float* __restrict__ partials,
                                                               float* __restrict__ ml) {
-  constexpr int LX = HD / 4, SL = 128 / LX;  // float4 columns, slices over the pieces
+  constexpr int KT = tile_of(HD), LX = HD / 4, SL = 128 / LX;  // float4 columns, slices over the pieces
   __shared__ int red[2][4];
   __shared__ float4 acc[SL][LX];
-  __shared__ float accl[SL];
+  __shared__ float accl[SL], redm[4];
   const int b = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = nq / c.kv_heads, kvh = head / G, ht = (head % G) / 16, row = (head % G) % 16;
   const int H = c.kv_heads * HT;
   pdl_wait();
   int before = 0, total = 0;
   for (int i = tid; i < c.seqs; i += 128) {
-    const int n = (clamped_len(c, lens, i) + kTile - 1) / kTile * H;
+    const int n = (clamped_len(c, lens, i) + KT - 1) / KT * H;
     total += n;
     if (i < b) before += n;
   }
@@ -518,7 +620,7 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const PagedCache c
   __syncthreads();
   total = red[0][0] + red[0][1] + red[0][2] + red[0][3];
   before = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  const int nt = (clamped_len(c, lens, b) + kTile - 1) / kTile;
+  const int nt = (clamped_len(c, lens, b) + KT - 1) / KT;
   uint16_t* dst = out + (int64_t(b) * nq + head) * HD;
   if (nt == 0) {
     if (tid < HD / 2) reinterpret_cast<uint32_t*>(dst)[tid] = 0u;
@@ -533,10 +635,16 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const PagedCache c
   auto piece = [&](int i) { return partials + int64_t(i == 0 ? first : 2 * (w0 + i)) * kPiece; };
   const int x = tid % LX, s = tid / LX;
   float mx = -INFINITY;
-  for (int i = 0; i < pieces; ++i) mx = fmaxf(mx, __ldcg(piece(i) + 16 * HD + 2 * row));
+  for (int i = tid; i < pieces; i += 128) mx = fmaxf(mx, __ldcg(piece(i) + 16 * HD + 2 * row));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+  if (lane == 0) redm[warp] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
   const float base = mx == -INFINITY ? 0.0f : mx;
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f;
+#pragma unroll 4
   for (int i = s; i < pieces; i += SL) {
     const float* p = piece(i);
     const float2 e = __ldcg(reinterpret_cast<const float2*>(p + 16 * HD + 2 * row));
@@ -736,10 +844,10 @@ template <bool F16, int HD, bool TWO, bool WEIGHTS>
 cudaError_t attn(const PagedCache& c, const PagedAttn& a, const PagedAttnWorkspace& w, int sms, cudaStream_t s) {
   const int HT = (a.nq / c.kv_heads + 15) / 16;
   auto kern = paged_attn_kernel<F16, HD, TWO, WEIGHTS>;
-  const size_t smem = size_t(kAttnWarps) * 24576 + (2 * size_t(c.seqs) + 1) * 4;
+  const size_t smem = size_t(kAttnWarps) * kUnits * kUnit + (2 * size_t(c.seqs) + 1) * 4;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  const int ctas = sms * kAttnCtasPerSm;
+  const int ctas = sms * attn_ctas(HD, TWO);
   kern<<<ctas, kAttnWarps * 32, smem, s>>>(c, a.q, a.sqb, a.sqh, a.lens, a.out, a.nq, HT, a.scale * 1.4426950408889634f,
                                            w.partials, w.logits, w.logit_stride, w.ml);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
@@ -770,9 +878,9 @@ void paged_set_page_size(PagedCache* c, int page_size) {
 
 size_t paged_attn_workspace(int seqs, int nq, int head_dim, int capacity, bool weights, int sms, void* base,
                             PagedAttnWorkspace* w) {
-  const size_t pieces = size_t(sms) * kAttnCtasPerSm * kAttnWarps * 2;
+  const size_t pieces = size_t(sms) * attn_ctas(64, false) * kAttnWarps * 2;
   const size_t b0 = up256(pieces * 16 * (head_dim + 2) * 4);
-  const int64_t stride = (int64_t(capacity) + kTile - 1) / kTile * kTile;
+  const int64_t stride = (int64_t(capacity) + tile_of(head_dim) - 1) / tile_of(head_dim) * tile_of(head_dim);
   const size_t b1 = weights ? up256(size_t(seqs) * nq * size_t(stride) * 4) : 0;
   const size_t b2 = weights ? up256(size_t(seqs) * nq * 8) : 0;
   if (w) {
@@ -787,7 +895,7 @@ size_t paged_attn_workspace(int seqs, int nq, int head_dim, int capacity, bool w
 
 int64_t paged_attn_tiles(const PagedCache& c, int nq) {
   const int64_t ht = (nq / c.kv_heads + 15) / 16;
-  return int64_t(c.seqs) * ((int64_t(c.capacity) + kTile - 1) / kTile) * c.kv_heads * ht;
+  return int64_t(c.seqs) * ((int64_t(c.capacity) + tile_of(c.head_dim) - 1) / tile_of(c.head_dim)) * c.kv_heads * ht;
 }
 
 cudaError_t launch_paged_attn(const PagedCache& c, const PagedAttn& a, const PagedAttnWorkspace& w, int sms,

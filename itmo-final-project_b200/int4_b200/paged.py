@@ -16,8 +16,6 @@ reference, whose decode benchmark uses transformers' StaticCache (``benchmarks/e
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -49,7 +47,7 @@ def _table(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be an int32 tensor [sequences, pages] with unit stride along the pages")
 
 
-def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> _lib.PagedCacheStruct:
+def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> bytes:
     _need(k.dim() == 4 and k.shape == v.shape, "k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim]")
     _need(k.dtype in _HALF and v.dtype == k.dtype, "k_cache and v_cache must both be bfloat16 or both float16")
     _table(table, "block_table")
@@ -59,7 +57,7 @@ def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> _lib.PagedC
     ks, vs = k.stride(), v.stride()
     _need(ks[3] == 1 and vs[3] == 1, "the caches' last dimension must have unit stride")
     seqs, width = table.shape
-    return _lib.PagedCacheStruct(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.data_ptr(),
+    return _lib.PAGED_CACHE.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.data_ptr(),
                                  table.stride(0), pages, heads, page, dim, seqs, width, _lib.DTYPE_CODE[k.dtype])
 
 
@@ -105,7 +103,7 @@ def paged_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos
     _on_gpu(dev, k_cache, v_cache, block_table, cos, sin, positions, slots, seqs, out)
     qkv = _rows16(qkv)
     with _lib.on_device(dev):
-        st = _lib.lib().i4b_paged_kv_append(ctypes.byref(c), qkv.data_ptr(), qkv.stride(0), T, nq, cos.data_ptr(),
+        st = _lib.lib().i4b_paged_kv_append(c, qkv.data_ptr(), qkv.stride(0), T, nq, cos.data_ptr(),
                                             sin.data_ptr(), _lib.DTYPE_CODE[cos.dtype], cos.shape[0],
                                             positions.data_ptr(), slots.data_ptr(),
                                             None if seqs is None else seqs.data_ptr(), out.data_ptr(),
@@ -136,7 +134,7 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
               and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1),
               f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
     if out is None:
-        out = torch.empty((B, nq, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _need(out.shape == (B, nq, dim) and out.dtype == q.dtype and out.is_contiguous(),
               "out must be a contiguous [sequences, nq, head_dim] of the caches' dtype")
@@ -148,7 +146,7 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         need = L.i4b_paged_attention_workspace_size(B, nq, nkv, dim, width * page, weights is not None)
         # from torch's allocator each time: two captured graphs never share it, and eager streams do not either
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        st = L.i4b_paged_decode_attention(ctypes.byref(c), q.data_ptr(), q.stride(0), q.stride(1), nq, lens.data_ptr(),
+        st = L.i4b_paged_decode_attention(c, q.data_ptr(), q.stride(0), q.stride(1), nq, lens.data_ptr(),
                                           dim ** -0.5 if scale is None else scale, out.data_ptr(),
                                           None if weights is None else weights.data_ptr(),
                                           0 if weights is None else weights.stride(0),
@@ -190,7 +188,7 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
     new_lens = torch.empty(B, dtype=torch.int32, device=dev)
     kept = torch.empty((B, nkv, budget), dtype=torch.int32, device=dev)
     with _lib.on_device(dev):
-        st = _lib.lib().i4b_paged_evict(ctypes.byref(c), weights.data_ptr(), weights.stride(0), weights.stride(1),
+        st = _lib.lib().i4b_paged_evict(c, weights.data_ptr(), weights.stride(0), weights.stride(1),
                                         weights.shape[2], lens.data_ptr(), new_table.data_ptr(), new_table.stride(0),
                                         new_table.shape[1], budget, recent, new_lens.data_ptr(), kept.data_ptr(),
                                         weights_out.data_ptr(), weights_out.stride(0), weights_out.stride(1),

@@ -1,8 +1,6 @@
 """What the paged-cache operators and token_logprobs refuse, before any CUDA call: no GPU needed."""
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 import torch
 
@@ -97,11 +95,12 @@ def _struct(**kw):
     d = dict(k=0x1000, v=0x2000, k_stride_page=2048, k_stride_head=1024, k_stride_token=64, v_stride_page=2048, v_stride_head=1024,
              v_stride_token=64, block_table=0x3000, table_stride=3, num_pages=6, kv_heads=2, page_size=16, head_dim=64, seqs=2,
              max_pages=3, dtype=1)
-    return _lib.PagedCacheStruct(**{**d, **kw})
+    d = {**d, **kw}
+    return _lib.PAGED_CACHE.pack(*(0 if x is None else x for x in d.values()))
 
 
 def _c_attend(cache, nq=8, q=0x4000, weights=None, ws=0x7000, size=1 << 40):
-    return _lib.lib().i4b_paged_decode_attention(ctypes.byref(cache), q, nq * 64, 64, nq, 0x5000, 0.125, 0x6000, weights, 96, 48, ws, size, None)
+    return _lib.lib().i4b_paged_decode_attention(cache, q, nq * 64, 64, nq, 0x5000, 0.125, 0x6000, weights, 96, 48, ws, size, None)
 
 
 @pytest.mark.parametrize("change, status", [
@@ -122,13 +121,13 @@ def test_c_statuses_of_the_other_arguments():
     c = _struct()
 
     def append(tokens=2, nq=8, table_dtype=2, max_pos=32, qkv=0x4000, stride=768, cos=0x8000):
-        return L.i4b_paged_kv_append(ctypes.byref(c), qkv, stride, tokens, nq, cos, 0x9000, table_dtype, max_pos, 0x5000, 0x5100, None, 0x6000, None)
+        return L.i4b_paged_kv_append(c, qkv, stride, tokens, nq, cos, 0x9000, table_dtype, max_pos, 0x5000, 0x5100, None, 0x6000, None)
 
     assert append(table_dtype=0) == 1 and append(tokens=-1) == 2 and append(nq=0) == 2 and append(max_pos=0) == 2
     assert append(qkv=None) == 1 and append(stride=770) == 4 and append(cos=0x8004) == 4 and append(tokens=0) == 0
 
     def evict(width=48, new_pages=2, budget=32, recent=0, weights=0x4000):
-        return L.i4b_paged_evict(ctypes.byref(c), weights, 96, 48, width, 0x5000, 0x5100, 2, new_pages, budget, recent, 0x6000, 0x6100,
+        return L.i4b_paged_evict(c, weights, 96, 48, width, 0x5000, 0x5100, 2, new_pages, budget, recent, 0x6000, 0x6100,
                                  0x6200, 96, 48, None)
 
     assert evict(width=47) == 2 and evict(new_pages=1) == 2 and evict(budget=0) == 2 and evict(recent=33) == 2 and evict(weights=None) == 1
