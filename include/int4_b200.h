@@ -288,7 +288,7 @@ int i4b_argmax_rows(const void* x, int64_t rows, int64_t n, int64_t* out, void* 
  * pages (its rotary angle is a matter of i4b_paged_kv_append alone, so slots may be compacted).
  *
  * Element (page, head, token, d) of the keys is at k + page * k_stride_page + head * k_stride_head +
- * token * k_stride_token + d, the same with v; strides are in elements and multiples of 8, bases 16-byte aligned, so
+ * token * k_stride_token + d, the same with v; strides are in elements and multiples of 8 (a token stride below 2^31), bases 16-byte aligned, so
  * both [pages, kv_heads, page_size, head_dim] and [pages, page_size, kv_heads, head_dim] memory will do.
  * block_table[seq * table_stride + i] is the page of slots i * page_size ...; an entry outside [0, num_pages) that a
  * length reaches is a page that holds nothing: its slots are left out of the attention, and nothing is written there.

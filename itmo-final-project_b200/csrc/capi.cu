@@ -572,12 +572,12 @@ int paged_cache(const i4b_paged_cache* in, PagedCache* c) {
   const int64_t extent[] = {in->num_pages, in->kv_heads, in->page_size};
   for (int i = 0; i < 6; ++i) {
     if (extent[i % 3] == 1) st[i] = 0;  // never used: whatever the caller's view says
-    if (st[i] < 0 || st[i] % 8 != 0) return I4B_ERR_LAYOUT;
+    if (st[i] < 0 || st[i] % 8 != 0 || (i % 3 == 2 && st[i] > INT32_MAX)) return I4B_ERR_LAYOUT;
   }
   c->k = static_cast<uint16_t*>(in->k);
   c->v = static_cast<uint16_t*>(in->v);
-  c->ks_page = st[0], c->ks_head = st[1], c->ks_token = st[2];
-  c->vs_page = st[3], c->vs_head = st[4], c->vs_token = st[5];
+  c->ks_page = st[0], c->ks_head = st[1], c->ks_token = int(st[2]);
+  c->vs_page = st[3], c->vs_head = st[4], c->vs_token = int(st[5]);
   c->table = in->block_table;
   c->table_stride = in->table_stride;
   c->seqs = int(in->seqs);
@@ -622,7 +622,8 @@ size_t i4b_paged_attention_workspace_size(int64_t seqs, int64_t nq, int64_t kv_h
     return 0;
   DevInfo d;
   if (current_device_info(&d)) return 0;
-  return paged_attn_workspace(int(seqs), int(nq), int(head_dim), int(capacity), with_weights != 0, d.sms, nullptr, nullptr);
+  return paged_attn_workspace(int(seqs), int(nq), int(kv_heads), int(head_dim), int(capacity), with_weights != 0, d.sms,
+                              nullptr, nullptr);
 }
 
 int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int64_t stride_qb, int64_t stride_qh,
@@ -631,7 +632,7 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
                                void* stream) {
   PagedCache c;
   if (int st = paged_cache(cache, &c)) return st;
-  if (nq <= 0 || nq > 65535 || nq % c.kv_heads != 0 || paged_attn_tiles(c, int(nq)) > INT32_MAX) return I4B_ERR_SHAPE;
+  if (nq <= 0 || nq > 65535 || nq % c.kv_heads != 0 || paged_attn_tiles(c, int(nq)) > (1 << 30)) return I4B_ERR_SHAPE;
   if (c.seqs == 0) return I4B_OK;
   if (!q || !lens || !out || !workspace) return I4B_ERR_INVALID_ARG;
   if (c.seqs == 1) stride_qb = 0;  // never used
@@ -641,7 +642,8 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
   DevInfo d;
   if (int st = current_device_info(&d)) return st;
   PagedAttnWorkspace w;
-  if (workspace_bytes < paged_attn_workspace(c.seqs, int(nq), c.head_dim, c.capacity, weights != nullptr, d.sms, workspace, &w))
+  if (workspace_bytes < paged_attn_workspace(c.seqs, int(nq), c.kv_heads, c.head_dim, c.capacity, weights != nullptr, d.sms,
+                                             workspace, &w))
     return I4B_ERR_WORKSPACE;
   const PagedAttn a = {static_cast<const uint16_t*>(q), stride_qb, stride_qh, lens, static_cast<uint16_t*>(out), int(nq),
                        scale, weights, stride_wb, stride_wh};

@@ -169,7 +169,8 @@ void set_decode_trace(void* buf, size_t bytes);
 struct PagedCache {  // strides in elements; the last dimension (head_dim) is contiguous
   uint16_t* k;
   uint16_t* v;
-  int64_t ks_page, ks_head, ks_token, vs_page, vs_head, vs_token;
+  int64_t ks_page, ks_head, vs_page, vs_head;
+  int ks_token, vs_token;
   const int32_t* table;
   int64_t table_stride;
   int seqs, capacity;  // rows of the table; positions that a row's pages hold
@@ -193,6 +194,8 @@ struct PagedAttnWorkspace {
   float* logits;
   int64_t logit_stride;
   float* ml;
+  int* counter;  // null: no shared runs
+  int* starts;
 };
 struct PagedEvict {
   const float* weights;
@@ -208,9 +211,9 @@ struct PagedEvict {
 };
 void paged_set_page_size(PagedCache* c, int page_size);
 // Bytes of the attention workspace; fills *w with its parts at `base` when w is not null.
-size_t paged_attn_workspace(int seqs, int nq, int head_dim, int capacity, bool weights, int sms, void* base,
-                            PagedAttnWorkspace* w);
-int64_t paged_attn_tiles(const PagedCache& c, int nq);  // at full length: has to fit 31 bits
+size_t paged_attn_workspace(int seqs, int nq, int kv_heads, int head_dim, int capacity, bool weights, int sms,
+                            void* base, PagedAttnWorkspace* w);
+int64_t paged_attn_tiles(const PagedCache& c, int nq);  // at full length: at most 2^30
 cudaError_t launch_paged_attn(const PagedCache& c, const PagedAttn& a, const PagedAttnWorkspace& w, int sms,
                               cudaStream_t s);
 cudaError_t launch_paged_append(const PagedCache& c, const uint16_t* qkv, int64_t sqkv, int64_t tokens, const void* cosT,

@@ -20,6 +20,10 @@ namespace i4b {
 
 namespace {
 
+__device__ __forceinline__ void cp_async_all(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -147,11 +151,14 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedCache c, c
 // ------------------------------------------------------------------ attention
 
 // The cached positions of every (sequence, kv head, 16 query heads) item are cut into tiles; the items' tiles, one item
-// behind the other, are dealt in equal consecutive runs to the grid's warps, each of which works by itself.  A run that
-// holds an item whole writes its output; the pieces of an item that several runs share go to the workspace as (max,
-// sum, unnormalised output) and paged_attn_join adds them in the runs' order.  The deal depends on the lengths alone,
-// so results repeat bit by bit.
+// behind the other, are cut into runs of consecutive tiles for the grid's warps, each of which works by itself.  A run
+// that holds an item whole writes its output; the pieces of an item that several runs share go to the workspace as
+// (max, sum, unnormalised output) and paged_attn_join adds them in the runs' order.  Where the runs begin depends on
+// the lengths alone, so results repeat bit by bit, whichever warp takes which run.
 //
+// Every warp has one run of its own; when there is much to do, that is 5/8 of its share, and the rest lies in short
+// runs that warps take from a counter: with equal shares alone the SMs, which do not see equal bandwidth, finished
+// between 77 and 127 us (687 MB, mean 103).
 // Both products are taken with the positions (or the head's dims) as the rows of the matrix instruction and the query
 // heads as its 8 columns -- S^T = K Q^T, O^T = V^T P^T -- so that a group of 4 or 8 query heads fills half or all of
 // it, not a quarter or half of 16 rows.  Between them P^T goes through an 8 x 8 transposition of registers.
@@ -171,22 +178,43 @@ __host__ __device__ constexpr int attn_ctas(int head_dim, bool two) { return two
 
 __host__ __device__ constexpr int tile_of(int head_dim) { return kUnit / 2 / head_dim; }  // 32 or 16 positions
 
+// A piece of an item in the workspace: the outputs of its query heads, then (max, sum) of each; 16-byte aligned.
+__host__ __device__ constexpr int piece_floats(int rows, int head_dim) { return rows * head_dim + (2 * rows + 3) / 4 * 4; }
+
 __device__ __forceinline__ int clamped_len(const PagedCache& c, const int32_t* lens, int b) {
   const int n = __ldg(lens + b);
   return n < 0 ? 0 : (n > c.capacity ? c.capacity : n);  // never reads past the table
 }
 
-__device__ __forceinline__ int run_tiles(int total, int workers) {
-  const int per = (total + workers - 1) / workers;
-  return per < kMinTiles ? kMinTiles : per;
-}
+// How `total` tiles are cut: run r < workers is tiles [r * own, + own), run workers + i is [workers * own + i * more, + more).
+constexpr int kSharedFrom = 16;  // tiles per warp from which on runs are shared
+
+struct Deal {
+  int total, workers, own, more;
+  __device__ Deal(int total_, int workers_, bool shared) : total(total_), workers(workers_) {
+    const int per = max((total + workers - 1) / workers, kMinTiles);
+    const bool both = shared && per >= kSharedFrom;
+    own = both ? per * 5 / 8 : per;
+    more = both ? max(4, per / 8) : 0;  // 3 short runs or so per warp, never shorter than what is requested ahead
+  }
+  __device__ int64_t first(int r) const {
+    return r < workers ? int64_t(r) * own : int64_t(workers) * own + int64_t(r - workers) * more;
+  }
+  __device__ int tiles(int r) const { return int(min(int64_t(r < workers ? own : more), total - first(r))); }
+  __device__ int run_of(int tile) const {
+    return tile < int64_t(workers) * own ? tile / own : workers + int((tile - int64_t(workers) * own) / more);
+  }
+};
+
+// Runs per worker that a Deal makes at most: its own, and (3/8 per + 1) / max(4, per / 8) < 4 short ones.
+constexpr int kMostRuns = 5;
 
 template <bool F16, int HD, bool TWO, bool WEIGHTS>
 __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
     paged_attn_kernel(const PagedCache c, const uint16_t* __restrict__ q, int64_t sqb, int64_t sqh,
                       const int32_t* __restrict__ lens, uint16_t* __restrict__ out, int nq, int HT, float scale_log2,
                       float* __restrict__ partials, float* __restrict__ logits, int64_t logit_stride,
-                      float* __restrict__ ml) {
+                      float* __restrict__ ml, int* __restrict__ counter, int* __restrict__ starts) {
   constexpr int KT = tile_of(HD);         // positions of a tile
   constexpr int KI = KT / 16, KR = KT / 8; // blocks of 16 positions; key rows that a lane owns
   constexpr int HC = HD / 32;              // 16-byte chunks of a key row that a lane uses: t + 4h
@@ -198,7 +226,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
   // 2t + 9 of every block).  Key word (row j, chunk t + 4h) of lane (g, t) lies at 32 (HC j + h) + ((4g + t) ^ 4 (h & 1)),
   // value word (row j, chunk g + 8v) at 32 (VC j + v) + 8t + (g ^ 2t).
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ int scan_tmp[kAttnWarps];
+  __shared__ int scan_tmp[kAttnWarps], queue[kAttnWarps][2][4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint4* ring = reinterpret_cast<uint4*>(smem + warp * (kUnits * kUnit));
   int* pre = reinterpret_cast<int*>(smem + kAttnWarps * kUnits * kUnit);  // [B + 1] first tile of each sequence
@@ -236,31 +264,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
     if (tid == 0) pre[B] = base;
     __syncthreads();
   }
-  const int total = pre[B];
-  const int workers = int(gridDim.x) * kAttnWarps, worker = int(blockIdx.x) * kAttnWarps + warp;
-  const int per = run_tiles(total, workers);
-  const int64_t begin64 = int64_t(worker) * per;
-  if (begin64 >= total) return;
-  const int begin = int(begin64), ntiles = min(per, total - begin);
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= B; b += kAttnWarps * 32) starts[b] = pre[b];  // for the join
+  const int worker = int(blockIdx.x) * kAttnWarps + warp;
+  const Deal deal(pre[B], int(gridDim.x) * kAttnWarps, counter != nullptr);
 
   struct Item {
     int b, h, len, nt;  // sequence; kv head and tile of query heads; the sequence's length and tiles
   };
-  Item ci;     // the item being computed, and its tile
-  int ctile;
-  {
-    int lo = 0, hi = B;  // pre[lo] <= begin < pre[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pre[mid] <= begin) lo = mid; else hi = mid;
-    }
-    ci.b = lo;
-    ci.len = len[lo];
-    ci.nt = (ci.len + KT - 1) / KT;
-    const int off = begin - pre[lo];
-    ci.h = off / ci.nt;
-    ctile = off - ci.h * ci.nt;
-  }
   auto next_item = [&](Item& x) {
     if (++x.h < H) return;
     x.h = 0;
@@ -274,8 +285,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
 
   // ---- requests.  Tile x's keys are requested after the values of tile x - 2 have been used, its values after the
   // keys of tile x - 1; its page numbers are read half a tile before that.
-  Item ri = ci;    // the item being requested, its tile, and what is the same for all its tiles
-  int rtile = ctile;
+  Item ri = {};          // the item being requested, its tile, and what is the same for all its tiles
+  int rtile, rleft = 0;  // and the tiles left in the run
   const int32_t* rtable;
   const uint16_t *rk, *rv;
   auto enter = [&]() {
@@ -284,105 +295,127 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
     rk = c.k + kvh * c.ks_head + 8 * (lane & 7);
     rv = c.v + kvh * c.vs_head + 8 * (lane & 7);
   };
-  enter();
-  // this lane copies chunk lane % 8 (+ 8y) of the key rows from KR * (4x + lane / 8), x = 0, 1, and of the value rows
-  // from 2 KR * (lane / 8)
-  const int lq = lane >> 3, l8 = lane & 7;
-  const int kdst = 32 * (l8 >> 2) + ((4 * lq + (l8 & 3)) ^ (4 * (l8 >> 2))), vdst = 8 * lq + (l8 ^ (2 * lq));
-  int requested = 0;   // tiles whose keys were requested
-  int kpage[2], krow[2], vpage = -1, vrow = 0;
-  krow[0] = krow[1] = 0;
-  auto fetch_pages = [&]() {
-    kpage[0] = kpage[1] = vpage = -1;
-    if (requested >= ntiles) return;
-    const int vpos = rtile * KT + 2 * KR * lq;
-    if (vpos < ri.len) {
-      const int pi = page_of(c, vpos);
-      vrow = vpos - pi * c.page_size;
-      vpage = __ldg(rtable + pi);
+  int ahead = 0;            // (lane 0) the short run that this warp takes next
+  auto take = [&](int r) {  // begin to request run r, if there is one
+    rleft = deal.tiles(r);
+    if (rleft <= 0) return;
+    if (deal.more > 0 && lane == 0) ahead = deal.workers + atomicAdd(counter, 1);
+    const int begin = int(deal.first(r));
+    int lo = 0, hi = B;  // pre[lo] <= begin < pre[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= begin) lo = mid; else hi = mid;
     }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int kpos = rtile * KT + KR * (4 * x + lq);
-      if (kpos < ri.len) {
-        const int pi = page_of(c, kpos);
-        krow[x] = kpos - pi * c.page_size;
-        kpage[x] = __ldg(rtable + pi);
-      }
+    ri.b = lo;
+    ri.len = len[lo];
+    ri.nt = (ri.len + KT - 1) / KT;
+    const int off = begin - pre[lo];
+    ri.h = off / ri.nt;
+    rtile = off - ri.h * ri.nt;
+    enter();
+  };
+  take(worker);
+  if (rleft <= 0) return;
+  Item ci = ri;  // the item being computed, its tile, the tiles left in its run, and the run
+  int ctile = rtile, cleft = rleft, run = worker, taken = 0, entered = 0;
+  // this lane copies chunk lane % 8 (+ 8y) of rows 2 KR (lane / 8) + j, j < 2 KR, keys and values alike: one page
+  const int lq = lane >> 3, l8 = lane & 7;
+  const int kdst = 32 * (l8 >> 2) + 8 * lq + ((l8 & 3) ^ (4 * (l8 >> 2))), vdst = 8 * lq + (l8 ^ (2 * lq));
+  int requested = 0;  // tiles whose keys were requested
+  int page = -1, row = 0;
+  auto fetch_page = [&]() {
+    page = -1;
+    const int pos = rtile * KT + 2 * KR * lq;
+    if (rleft > 0 && pos < ri.len) {
+      const int pi = page_of(c, pos);
+      row = pos - pi * c.page_size;
+      page = __ldg(rtable + pi);
     }
   };
-  const uint16_t* vsrc = nullptr;  // the first of the value rows of the tile whose values are requested next
-  int vleft = 0;                   // how many of them exist
-  uint32_t flags = 0;  // two bits for each of the last tiles (x & 7): every position there; this lane's key page there
+  const uint16_t* vsrc = nullptr;  // the first of the rows of the tile whose values are requested next
+  int left = 0;                    // how many of them exist
+  uint32_t flags = 0;  // two bits for each of the last tiles (x & 7): every position there; the page of key rows KR g there
   auto request_keys = [&](uint4* dst) {
     __syncwarp();  // the slot has been read by every lane
-    if (requested < ntiles) {
-      const bool ok0 = uint32_t(kpage[0]) < uint32_t(c.num_pages), ok1 = uint32_t(kpage[1]) < uint32_t(c.num_pages);
-      const bool vok = uint32_t(vpage) < uint32_t(c.num_pages);
-      const uint32_t b0 = __ballot_sync(0xFFFFFFFFu, ok0), b1 = __ballot_sync(0xFFFFFFFFu, ok1);
-      const bool full = (rtile + 1) * KT <= ri.len && (b0 & b1) == 0xFFFFFFFFu;  // (a tile's values have its keys' pages)
-      const uint32_t f = (full ? 1u : 0u) | ((g & 4 ? b1 : b0) >> (8 * (g & 3)) & 1u) << 1;
+    if (rleft > 0) {
+      const bool ok = uint32_t(page) < uint32_t(c.num_pages);
+      const uint32_t oks = __ballot_sync(0xFFFFFFFFu, ok);
+      const bool full = (rtile + 1) * KT <= ri.len && oks == 0xFFFFFFFFu;
       const int sh = (requested & 7) * 2;
-      flags = (flags & ~(3u << sh)) | (f << sh);
-      vsrc = rv + vpage * c.vs_page + vrow * c.vs_token;
-      vleft = vok ? ri.len - (rtile * KT + 2 * KR * lq) : 0;
+      flags = (flags & ~(3u << sh)) | ((full ? 1u : 0u) | (oks >> (8 * (g >> 1)) & 1u) << 1) << sh;
+      vsrc = rv + page * c.vs_page + int64_t(row) * c.vs_token;
+      left = ok ? ri.len - (rtile * KT + 2 * KR * lq) : 0;
+      const uint16_t* src = rk + page * c.ks_page + int64_t(row) * c.ks_token;
+      if (full) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint16_t* src = rk + kpage[x] * c.ks_page + krow[x] * c.ks_token;
-        const int left = (x ? ok1 : ok0) ? ri.len - (rtile * KT + KR * (4 * x + lq)) : 0;
+        for (int j = 0; j < 2 * KR; ++j, src += c.ks_token)
 #pragma unroll
-        for (int j = 0; j < KR; ++j, src += c.ks_token)
+          for (int y = 0; y < HC / 2; ++y)
+            cp_async_all(dst + 32 * (HC * (j % KR) + 2 * y) + (kdst ^ (4 * (j / KR))), src + 64 * y);
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < 2 * KR; ++j, src += c.ks_token)
 #pragma unroll
-          for (int y = 0; y < HC / 2; ++y) {
-            uint4* to = dst + 32 * (HC * j + 2 * y) + (kdst ^ (16 * x));
-            if (full)
-              cp_async_16(to, src + 64 * y, 16u);
-            else
-              cp_async_16(to, j < left ? src + 64 * y : c.k, j < left ? 16u : 0u);
-          }
+          for (int y = 0; y < HC / 2; ++y)
+            cp_async_16(dst + 32 * (HC * (j % KR) + 2 * y) + (kdst ^ (4 * (j / KR))), j < left ? src + 64 * y : c.k,
+                        j < left ? 16u : 0u);
       }
       ++requested;
-      if (++rtile == ri.nt) {
+      ++rtile;
+      if (--rleft == 0) {
+        if (deal.more > 0) {  // left for the computation, which is two tiles behind: at most two runs wait there
+          const int r = __shfl_sync(0xFFFFFFFFu, ahead, 0);
+          take(r);
+          if (lane == 0) {
+            int* to = queue[warp][taken & 1];
+            to[0] = rleft > 0 ? r : -1;
+            to[1] = ri.b, to[2] = ri.h, to[3] = rtile;
+          }
+          ++taken;
+        }
+      } else if (rtile == ri.nt) {
         rtile = 0;
         next_item(ri);
-        if (requested < ntiles) enter();
+        enter();
       }
     }
     cp_async_commit();
   };
   auto request_values = [&](uint4* dst, int x) {  // of tile x
     __syncwarp();
-    if (x < ntiles) {
-      const bool full = flags >> ((x & 7) * 2) & 1u;
+    if (x < requested) {
       const uint16_t* src = vsrc;
+      if (flags >> ((x & 7) * 2) & 1u) {
 #pragma unroll
-      for (int j = 0; j < 2 * KR; ++j, src += c.vs_token)
+        for (int j = 0; j < 2 * KR; ++j, src += c.vs_token)
 #pragma unroll
-        for (int v = 0; v < VC; ++v) {
-          uint4* to = dst + 32 * (VC * j + v) + vdst;
-          if (full)
-            cp_async_16(to, src + 64 * v, 16u);
-          else
-            cp_async_16(to, j < vleft ? src + 64 * v : c.v, j < vleft ? 16u : 0u);  // rows that do not exist: zeros
-        }
+          for (int v = 0; v < VC; ++v) cp_async_all(dst + 32 * (VC * j + v) + vdst, src + 64 * v);
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < 2 * KR; ++j, src += c.vs_token)
+#pragma unroll
+          for (int v = 0; v < VC; ++v)  // rows that do not exist arrive as zeros, whatever they hold
+            cp_async_16(dst + 32 * (VC * j + v) + vdst, j < left ? src + 64 * v : c.v, j < left ? 16u : 0u);
+      }
     }
     cp_async_commit();
   };
   constexpr int kSlot = kUnit / 16;
-  fetch_pages();
+  fetch_page();
   request_keys(ring);
   request_values(ring + kSlot, 0);
-  fetch_pages();
+  fetch_page();
   request_keys(ring + 2 * kSlot);
 
+  const int prows = min(16, G), piece = piece_floats(prows, HD);
   // A negative scale turns the queries' signs instead, so that the largest product has the largest score.
   const uint32_t flip = scale_log2 < 0.0f ? 0x80008000u : 0u;
   const float scl = fabsf(scale_log2);
   uint32_t qb[R][2 * HC][2];
   float o[R][4 * VC][4], m[R][2], l[R][2];  // of heads 2t and 2t + 1 of each block of 8
-  int slot = 0, seg_first = 0, seg_tile0 = ctile;
-  bool fresh = true;
-  for (int n = 0; n < ntiles; ++n) {
+  int slot = 0, seg_tile0 = ctile;
+  bool fresh = true, first_seg = true;  // of its run
+  for (int n = 0;; ++n) {
     if (fresh) {
       fresh = false;
       const int kvh = HT == 1 ? ci.h : ci.h / HT, head0 = kvh * G + (HT == 1 ? 0 : ci.h % HT) * 16;
@@ -428,18 +461,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
     }
     request_values(ring + slot * kSlot, n + 1);
     slot = slot == kUnits - 1 ? 0 : slot + 1;
-    fetch_pages();
+    fetch_page();
     // ---- softmax; the lane's scores are those of its key rows KR * g + KI * e + i, entries [i][2 * e + head]
     const uint32_t f = flags >> ((n & 7) * 2);
     if (!(f & 1u)) {
-      const int left = f >> 1 & 1u ? ci.len - (ctile * KT + KR * g) : 0;
+      const int there = f >> 1 & 1u ? ci.len - (ctile * KT + KR * g) : 0;
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int i = 0; i < KI; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (KI * e + i >= left) s[r][i][2 * e] = s[r][i][2 * e + 1] = -INFINITY;
+            if (KI * e + i >= there) s[r][i][2 * e] = s[r][i][2 * e + 1] = -INFINITY;
     }
     // The reference point m of the exponentials follows the maximum with a slack of 2^8: it moves, and what is summed
     // so far is scaled, only when a score passes it by more (and with a head's first score).
@@ -540,11 +573,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
     request_keys(ring + slot * kSlot);
     slot = slot == kUnits - 1 ? 0 : slot + 1;
     // ---- end of the item, or of this run
-    if (ctile == ci.nt - 1 || n == ntiles - 1) {
+    --cleft;
+    if (ctile == ci.nt - 1 || cleft == 0) {
       const int kvh = HT == 1 ? ci.h : ci.h / HT, head0 = kvh * G + (HT == 1 ? 0 : ci.h % HT) * 16;
       const int rows = min(16, kvh * G + G - head0);
       const bool whole = seg_tile0 == 0 && ctile == ci.nt - 1;
-      float* part = partials + int64_t(2 * worker + (seg_first == 0 ? 0 : 1)) * (16 * (HD + 2));
+      float* part = partials + int64_t(2 * run + (first_seg ? 0 : 1)) * piece;
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -574,15 +608,26 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
                 for (int i = 0; i < 4; i += 2)
                   *reinterpret_cast<float4*>(dst + 8 * (g + 8 * v) + 2 * i) =
                       make_float4(o[r][4 * v + i][u], o[r][4 * v + i][2 + u], o[r][4 * v + i + 1][u], o[r][4 * v + i + 1][2 + u]);
-              if (g == 0) *reinterpret_cast<float2*>(part + 16 * HD + 2 * row) = make_float2(m[r][u], ls);
+              if (g == 0) *reinterpret_cast<float2*>(part + HD * prows + 2 * row) = make_float2(m[r][u], ls);
             }
           }
         }
       fresh = true;
-      seg_first = n + 1;
+      first_seg = false;
       seg_tile0 = 0;
     }
-    if (++ctile == ci.nt) {
+    if (cleft == 0) {
+      if (deal.more == 0) break;
+      __syncwarp();
+      const int* from = queue[warp][entered++ & 1];
+      run = from[0];
+      if (run < 0) break;
+      ci.b = from[1], ci.h = from[2], ctile = seg_tile0 = from[3];
+      ci.len = len[ci.b];
+      ci.nt = (ci.len + KT - 1) / KT;
+      cleft = deal.tiles(run);
+      first_seg = true;
+    } else if (++ctile == ci.nt) {
       ctile = 0;
       next_item(ci);
     }
@@ -590,81 +635,94 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
   cp_async_wait<0>();
 }
 
-// One CTA per (sequence, query head): adds the pieces of an item that several runs share, in the runs' order, and
-// writes zeros for an empty sequence.
-template <bool F16, int HD>
-__global__ void __launch_bounds__(128) paged_attn_join_kernel(const PagedCache c, const int32_t* __restrict__ lens,
-                                                              uint16_t* __restrict__ out, int nq, int HT, int workers,
-                                                              const float* __restrict__ partials,
-                                                              float* __restrict__ ml) {
-  constexpr int KT = tile_of(HD), LX = HD / 4, SL = 128 / LX;  // float4 columns, slices over the pieces
-  __shared__ int red[2][4];
-  __shared__ float4 acc[SL][LX];
-  __shared__ float accl[SL], redm[4];
-  const int b = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = nq / c.kv_heads, kvh = head / G, ht = (head % G) / 16, row = (head % G) % 16;
-  const int H = c.kv_heads * HT;
+// A group of TPH threads per (sequence, query head): adds the pieces of an item that several runs share, in the runs'
+// order, and writes zeros for an empty sequence.  Most items of a large batch lie in one run and have nothing to add;
+// an item of few long sequences has hundreds of pieces, eight of which each thread has in flight.  TPH = 32 from 2048
+// heads on (8 of them in a CTA), 128 from 512 on, else 512 (one each).
+template <bool F16, int HD, int TPH>
+__global__ void __launch_bounds__(TPH == 32 ? 256 : TPH)
+    paged_attn_join_kernel(int seqs, int kv_heads, uint16_t* __restrict__ out, int nq, int HT, int workers, int shared,
+                           const int* starts, const float* partials, float* ml) {
+  constexpr int LX = HD / 4;                    // float4 columns
+  constexpr int SL = TPH > LX ? TPH / LX : 1;   // slices over the pieces
+  constexpr int CX = TPH > LX ? 1 : LX / TPH;   // columns per thread
+  constexpr int NW = TPH / 32;
+  static_assert(CX == 1, "a warp covers a head's outputs");
+  __shared__ float4 acc[TPH > 32 ? SL : 1][LX];
+  __shared__ float accl[TPH > 32 ? SL : 1], redm[NW];
+  const int64_t at = TPH == 32 ? int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  const int tid = threadIdx.x % TPH, lane = threadIdx.x & 31;
+  if (at >= int64_t(seqs) * nq) return;
+  const int b = int(at / nq), head = int(at - int64_t(b) * nq);
+  const int G = nq / kv_heads, kvh = head / G, ht = (head % G) / 16, row = (head % G) % 16, prows = min(16, G);
   pdl_wait();
-  int before = 0, total = 0;
-  for (int i = tid; i < c.seqs; i += 128) {
-    const int n = (clamped_len(c, lens, i) + KT - 1) / KT * H;
-    total += n;
-    if (i < b) before += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-    before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
-  }
-  if (lane == 0) red[0][warp] = total, red[1][warp] = before;
-  __syncthreads();
-  total = red[0][0] + red[0][1] + red[0][2] + red[0][3];
-  before = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  const int nt = (clamped_len(c, lens, b) + KT - 1) / KT;
-  uint16_t* dst = out + (int64_t(b) * nq + head) * HD;
+  const int start = __ldcg(starts + b), nt = (__ldcg(starts + b + 1) - start) / (kv_heads * HT);
+  const Deal deal(__ldcg(starts + seqs), workers, shared != 0);
+  uint16_t* dst = out + at * HD;
   if (nt == 0) {
-    if (tid < HD / 2) reinterpret_cast<uint32_t*>(dst)[tid] = 0u;
-    if (ml && tid == 0) *reinterpret_cast<float2*>(ml + 2 * (int64_t(b) * nq + head)) = make_float2(0.0f, 0.0f);
+    for (int i = tid; i < HD / 2; i += TPH) reinterpret_cast<uint32_t*>(dst)[i] = 0u;
+    if (ml && tid == 0) *reinterpret_cast<float2*>(ml + 2 * at) = make_float2(0.0f, 0.0f);
     return;
   }
-  const int per = run_tiles(total, workers);
-  const int t0 = before + (kvh * HT + ht) * nt, w0 = t0 / per, w1 = (t0 + nt - 1) / per;
-  if (w0 == w1) return;  // written by the run itself
-  const int first = 2 * w0 + (int64_t(w0) * per == t0 ? 0 : 1), pieces = w1 - w0 + 1;
-  constexpr int64_t kPiece = 16 * (HD + 2);
-  auto piece = [&](int i) { return partials + int64_t(i == 0 ? first : 2 * (w0 + i)) * kPiece; };
+  const int t0 = start + (kvh * HT + ht) * nt, r0 = deal.run_of(t0), r1 = deal.run_of(t0 + nt - 1);
+  if (r0 == r1) return;  // written by the run itself
+  const int first = 2 * r0 + (deal.first(r0) == t0 ? 0 : 1), pieces = r1 - r0 + 1;
+  auto piece = [&](int i) { return partials + int64_t(i == 0 ? first : 2 * (r0 + i)) * piece_floats(prows, HD); };
   const int x = tid % LX, s = tid / LX;
   float mx = -INFINITY;
-  for (int i = tid; i < pieces; i += 128) mx = fmaxf(mx, __ldcg(piece(i) + 16 * HD + 2 * row));
+#pragma unroll 4
+  for (int i = tid; i < pieces; i += TPH) mx = fmaxf(mx, __ldcg(piece(i) + prows * HD + 2 * row));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-  if (lane == 0) redm[warp] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
+  if constexpr (TPH > 32) {
+    if (lane == 0) redm[tid >> 5] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) mx = fmaxf(mx, redm[i]);
+  }
   const float base = mx == -INFINITY ? 0.0f : mx;
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f;
-#pragma unroll 4
-  for (int i = s; i < pieces; i += SL) {
-    const float* p = piece(i);
-    const float2 e = __ldcg(reinterpret_cast<const float2*>(p + 16 * HD + 2 * row));
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p + row * HD + 4 * x));
-    const float f = ex2(e.x - base);
-    a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
-    l = fmaf(e.y, f, l);
+  constexpr int kBatch = 8;
+  for (int i0 = s; i0 < pieces; i0 += kBatch * SL) {
+    float2 e[kBatch];
+    float4 v[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * SL;
+      if (i < pieces) {
+        const float* p = piece(i);
+        e[k] = __ldcg(reinterpret_cast<const float2*>(p + prows * HD + 2 * row));
+        v[k] = __ldcg(reinterpret_cast<const float4*>(p + row * HD + 4 * x));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (i0 + k * SL < pieces) {
+        const float f = ex2(e[k].x - base);
+        a.x = fmaf(v[k].x, f, a.x), a.y = fmaf(v[k].y, f, a.y), a.z = fmaf(v[k].z, f, a.z), a.w = fmaf(v[k].w, f, a.w);
+        l = fmaf(e[k].y, f, l);
+      }
   }
-  acc[s][x] = a;
-  if (x == 0) accl[s] = l;
-  __syncthreads();
-  if (s != 0) return;
-  for (int i = 1; i < SL; ++i) {
-    const float4 v = acc[i][x];
-    a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-    l += accl[i];
+  if constexpr (TPH > 32) {
+    acc[s][x] = a;
+    if (x == 0) accl[s] = l;
+    __syncthreads();
+    if (s != 0) return;
+    for (int i = 1; i < SL; ++i) {
+      const float4 v = acc[i][x];
+      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+      l += accl[i];
+    }
+  } else if constexpr (SL == 2) {
+    a.x += __shfl_xor_sync(0xFFFFFFFFu, a.x, 16), a.y += __shfl_xor_sync(0xFFFFFFFFu, a.y, 16);
+    a.z += __shfl_xor_sync(0xFFFFFFFFu, a.z, 16), a.w += __shfl_xor_sync(0xFFFFFFFFu, a.w, 16);
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, 16);
+    if (s != 0) return;
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   *reinterpret_cast<uint2*>(dst + 4 * x) = make_uint2(pack2<F16>(a.x * inv, a.y * inv), pack2<F16>(a.z * inv, a.w * inv));
-  if (ml && x == 0) *reinterpret_cast<float2*>(ml + 2 * (int64_t(b) * nq + head)) = make_float2(mx, inv);
+  if (ml && x == 0) *reinterpret_cast<float2*>(ml + 2 * at) = make_float2(mx, inv);
 }
 
 // weights[b, kvh, j] += sum over the kv head's query heads of exp2(s_j - m) / l, from the stored scaled scores.
@@ -847,12 +905,17 @@ cudaError_t attn(const PagedCache& c, const PagedAttn& a, const PagedAttnWorkspa
   const size_t smem = size_t(kAttnWarps) * kUnits * kUnit + (2 * size_t(c.seqs) + 1) * 4;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  const int ctas = sms * attn_ctas(HD, TWO);
+  const int ctas = sms * attn_ctas(HD, TWO), workers = ctas * kAttnWarps;
+  if (w.counter && (e = cudaMemsetAsync(w.counter, 0, sizeof(int), s)) != cudaSuccess) return e;
   kern<<<ctas, kAttnWarps * 32, smem, s>>>(c, a.q, a.sqb, a.sqh, a.lens, a.out, a.nq, HT, a.scale * 1.4426950408889634f,
-                                           w.partials, w.logits, w.logit_stride, w.ml);
+                                           w.partials, w.logits, w.logit_stride, w.ml, w.counter, w.starts);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  e = launch_after(paged_attn_join_kernel<F16, HD>, dim3(unsigned(a.nq), unsigned(c.seqs)), dim3(128), 0, s, c, a.lens,
-                   a.out, a.nq, HT, ctas * kAttnWarps, static_cast<const float*>(w.partials), w.ml);
+  const int64_t heads = int64_t(c.seqs) * a.nq;
+  auto join = heads >= 2048 ? paged_attn_join_kernel<F16, HD, 32>
+                            : (heads >= 512 ? paged_attn_join_kernel<F16, HD, 128> : paged_attn_join_kernel<F16, HD, 512>);
+  e = launch_after(join, dim3(unsigned(heads >= 2048 ? (heads + 7) / 8 : heads)), dim3(heads >= 2048 ? 256 : (heads >= 512 ? 128 : 512)),
+                   0, s, c.seqs, c.kv_heads, a.out, a.nq, HT, workers, w.counter ? 1 : 0,
+                   static_cast<const int*>(w.starts), static_cast<const float*>(w.partials), w.ml);
   if (e != cudaSuccess || !WEIGHTS || c.capacity == 0) return e;
   return launch_after(paged_attn_weights_kernel, dim3(unsigned((c.capacity + 1023) / 1024), unsigned(c.kv_heads), unsigned(c.seqs)),
                       dim3(256), 0, s, c, a.lens, a.nq, static_cast<const float*>(w.logits), w.logit_stride,
@@ -876,21 +939,27 @@ void paged_set_page_size(PagedCache* c, int page_size) {
   c->ps_shift = l - 1;
 }
 
-size_t paged_attn_workspace(int seqs, int nq, int head_dim, int capacity, bool weights, int sms, void* base,
-                            PagedAttnWorkspace* w) {
-  const size_t pieces = size_t(sms) * attn_ctas(64, false) * kAttnWarps * 2;
-  const size_t b0 = up256(pieces * 16 * (head_dim + 2) * 4);
-  const int64_t stride = (int64_t(capacity) + tile_of(head_dim) - 1) / tile_of(head_dim) * tile_of(head_dim);
-  const size_t b1 = weights ? up256(size_t(seqs) * nq * size_t(stride) * 4) : 0;
-  const size_t b2 = weights ? up256(size_t(seqs) * nq * 8) : 0;
+size_t paged_attn_workspace(int seqs, int nq, int kv_heads, int head_dim, int capacity, bool weights, int sms,
+                            void* base, PagedAttnWorkspace* w) {
+  const int G = nq / kv_heads, tile = tile_of(head_dim), HT = (G + 15) / 16;
+  const int64_t workers = int64_t(sms) * attn_ctas(head_dim, G > 8) * kAttnWarps;
+  const int64_t stride = (int64_t(capacity) + tile - 1) / tile * tile;
+  // the lengths are on the device: runs are shared where the tables' whole capacity would call for it
+  const bool shared = int64_t(seqs) * (stride / tile) * kv_heads * HT >= workers * kSharedFrom;
+  const int64_t pieces = 2 * workers * (shared ? kMostRuns : 1);
+  const size_t b0 = up256(size_t(pieces) * piece_floats(std::min(G, 16), head_dim) * 4), b1 = 256 + up256(4 * (size_t(seqs) + 1));
+  const size_t b2 = weights ? up256(size_t(seqs) * nq * size_t(stride) * 4) : 0;
+  const size_t b3 = weights ? up256(size_t(seqs) * nq * 8) : 0;
   if (w) {
     char* p = static_cast<char*>(base);
     w->partials = reinterpret_cast<float*>(p);
-    w->logits = weights ? reinterpret_cast<float*>(p + b0) : nullptr;
+    w->counter = shared ? reinterpret_cast<int*>(p + b0) : nullptr;
+    w->starts = reinterpret_cast<int*>(p + b0 + 256);
+    w->logits = weights ? reinterpret_cast<float*>(p + b0 + b1) : nullptr;
     w->logit_stride = stride;
-    w->ml = weights ? reinterpret_cast<float*>(p + b0 + b1) : nullptr;
+    w->ml = weights ? reinterpret_cast<float*>(p + b0 + b1 + b2) : nullptr;
   }
-  return b0 + b1 + b2;
+  return b0 + b1 + b2 + b3;
 }
 
 int64_t paged_attn_tiles(const PagedCache& c, int nq) {
