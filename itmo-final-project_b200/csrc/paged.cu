@@ -20,8 +20,15 @@ namespace i4b {
 
 namespace {
 
-__device__ __forceinline__ void cp_async_all(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// 16 bytes global -> shared of data that is read once: the first to leave L2, so that what this kernel writes stays.
+__device__ __forceinline__ uint64_t policy_evict_first() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void cp_async_once(void* dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "l"(policy)
+               : "memory");
 }
 
 __device__ __forceinline__ float ex2(float v) {
@@ -164,17 +171,20 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedCache c, c
 // it, not a quarter or half of 16 rows.  Between them P^T goes through an 8 x 8 transposition of registers.
 //
 // Bound by the bytes of K and V: the products are a few percent of what even mma.sync can do, so what counts is bytes
-// in flight and whole 128-byte lines for each quarter of a warp.  Each warp keeps three units of 4 KB (a tile's keys or
-// its values) on their way, as a queue of its own in shared memory: a quarter copies one row (or half of a 256-byte
+// in flight and whole 128-byte lines for each quarter of a warp.  Each warp keeps four units of 4 KB (two tiles' keys
+// and values) on their way, in shared memory of its own: a quarter copies one row (or half of a 256-byte
 // one), and the 16-byte words are placed so that neither that nor the reading of the MMA fragments meets a bank twice.
 // (With every lane copying just the words of its own fragments, which needs no exchange, the values came in 32-byte
-// pieces: 160 us against 129 for 687 MB.)
-constexpr int kAttnWarps = 4;
+// pieces: 160 us against 129 for 687 MB at that stage.)
+// Warps per CTA and CTAs per SM as measured (687 MB, fp16, head_dim 64; main kernel): 5 x 2 108 us, 7 x 1 107, 6 x 2 111,
+// 8 x 1 110, 6 x 1 112, 4 x 2 122, 4 x 3 123, 10 x 1 127; on 74 MB 5 x 2 is the fastest too (17.0 us; 7 x 1 20.2).
+constexpr int kAttnWarps = 5;
+constexpr int kAttnCtas = 2;
 constexpr int kUnit = 4096;  // bytes of a tile's keys, or values
-constexpr int kUnits = 3;    // in flight per warp
+constexpr int kUnits = 4;    // in flight per warp: keys and values of two tiles
 constexpr int kMinTiles = 2;
 
-__host__ __device__ constexpr int attn_ctas(int head_dim, bool two) { return two && head_dim == 128 ? 3 : 4; }  // per SM
+__host__ __device__ constexpr int attn_warp_smem(int head_dim, bool two) { return kUnits * kUnit + (two ? 2 : 1) * head_dim * 16; }
 
 __host__ __device__ constexpr int tile_of(int head_dim) { return kUnit / 2 / head_dim; }  // 32 or 16 positions
 
@@ -186,31 +196,49 @@ __device__ __forceinline__ int clamped_len(const PagedCache& c, const int32_t* l
   return n < 0 ? 0 : (n > c.capacity ? c.capacity : n);  // never reads past the table
 }
 
-// How `total` tiles are cut: run r < workers is tiles [r * own, + own), run workers + i is [workers * own + i * more, + more).
+// How `total` tiles are cut into runs.  The first `workers` runs are the warps' own: of `own` tiles, the first `longer`
+// of them of one more.  Where runs are shared, those of `more` tiles follow, and for the end ones of 2.
 constexpr int kSharedFrom = 16;  // tiles per warp from which on runs are shared
 
 struct Deal {
-  int total, workers, own, more;
+  int total, workers, own, longer, more, long_end, more_end, more_runs;  // tiles: end of the own runs' longer ones, of ...
   __device__ Deal(int total_, int workers_, bool shared) : total(total_), workers(workers_) {
-    const int per = max((total + workers - 1) / workers, kMinTiles);
-    const bool both = shared && per >= kSharedFrom;
-    own = both ? per * 5 / 8 : per;
-    more = both ? max(4, per / 8) : 0;  // 3 short runs or so per warp, never shorter than what is requested ahead
+    const int per = total / workers;
+    if (shared && per >= kSharedFrom) {
+      own = per * 5 / 8;
+      longer = 0;
+      more = max(4, per / 8);
+      more_runs = (total - workers * own - 2 * workers + more - 1) / more;  // (per - own >= 6; the last may end with the tiles)
+    } else {
+      own = max(per, kMinTiles);
+      longer = per >= kMinTiles ? total - workers * per : 0;
+      more = more_runs = 0;
+    }
+    long_end = longer * (own + 1);
+    more_end = workers * own + longer + more_runs * more;
   }
   __device__ int64_t first(int r) const {
-    return r < workers ? int64_t(r) * own : int64_t(workers) * own + int64_t(r - workers) * more;
+    if (r < workers) return int64_t(r) * own + min(r, longer);
+    r -= workers;
+    return r < more_runs ? int64_t(workers) * own + longer + int64_t(r) * more : more_end + 2 * int64_t(r - more_runs);
   }
-  __device__ int tiles(int r) const { return int(min(int64_t(r < workers ? own : more), total - first(r))); }
+  __device__ int tiles(int r) const {
+    const int n = r < workers ? own + (r < longer ? 1 : 0) : (more == 0 ? 0 : (r < workers + more_runs ? more : 2));
+    return int(min(int64_t(n), total - first(r)));
+  }
   __device__ int run_of(int tile) const {
-    return tile < int64_t(workers) * own ? tile / own : workers + int((tile - int64_t(workers) * own) / more);
+    if (tile < long_end) return tile / (own + 1);
+    if (tile < int64_t(workers) * own + longer) return longer + (tile - long_end) / own;
+    if (tile < more_end) return workers + (tile - workers * own - longer) / more;
+    return workers + more_runs + (tile - more_end) / 2;
   }
 };
 
-// Runs per worker that a Deal makes at most: its own, and (3/8 per + 1) / max(4, per / 8) < 4 short ones.
-constexpr int kMostRuns = 5;
+// Runs per worker that a Deal makes at most: its own, (3/8 per + 2) / max(4, per / 8) < 4 and just over 1 of two tiles.
+constexpr int kMostRuns = 7;
 
 template <bool F16, int HD, bool TWO, bool WEIGHTS>
-__global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
+__global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
     paged_attn_kernel(const PagedCache c, const uint16_t* __restrict__ q, int64_t sqb, int64_t sqh,
                       const int32_t* __restrict__ lens, uint16_t* __restrict__ out, int nq, int HT, float scale_log2,
                       float* __restrict__ partials, float* __restrict__ logits, int64_t logit_stride,
@@ -228,8 +256,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int scan_tmp[kAttnWarps], queue[kAttnWarps][2][4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint4* ring = reinterpret_cast<uint4*>(smem + warp * (kUnits * kUnit));
-  int* pre = reinterpret_cast<int*>(smem + kAttnWarps * kUnits * kUnit);  // [B + 1] first tile of each sequence
+  constexpr int kWarpSmem = attn_warp_smem(HD, TWO);
+  uint4* ring = reinterpret_cast<uint4*>(smem + warp * kWarpSmem);           // keys, keys, values, values, queries
+  int* pre = reinterpret_cast<int*>(smem + kAttnWarps * kWarpSmem);  // [B + 1] first tile of each sequence
   int* len = pre + c.seqs + 1;                                            // [B]
   const int H = c.kv_heads * HT, B = c.seqs, G = nq / c.kv_heads;
 
@@ -283,17 +312,19 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
     }
   };
 
-  // ---- requests.  Tile x's keys are requested after the values of tile x - 2 have been used, its values after the
-  // keys of tile x - 1; its page numbers are read half a tile before that.
+  // ---- requests.  A tile's keys and values are requested as soon as those two tiles before have been used; its page
+  // number is read half a tile before that, and an item's queries come with its first keys.
   Item ri = {};          // the item being requested, its tile, and what is the same for all its tiles
   int rtile, rleft = 0;  // and the tiles left in the run
   const int32_t* rtable;
   const uint16_t *rk, *rv;
+  int items = 0, used = 0, held = 0, asked = 0;  // items requested, computed; whose queries are in shared memory, asked for
   auto enter = [&]() {
     const int kvh = HT == 1 ? ri.h : ri.h / HT;
     rtable = c.table + int64_t(ri.b) * c.table_stride;
     rk = c.k + kvh * c.ks_head + 8 * (lane & 7);
     rv = c.v + kvh * c.vs_head + 8 * (lane & 7);
+    ++items;
   };
   int ahead = 0;            // (lane 0) the short run that this warp takes next
   auto take = [&](int r) {  // begin to request run r, if there is one
@@ -321,6 +352,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
   // this lane copies chunk lane % 8 (+ 8y) of rows 2 KR (lane / 8) + j, j < 2 KR, keys and values alike: one page
   const int lq = lane >> 3, l8 = lane & 7;
   const int kdst = 32 * (l8 >> 2) + 8 * lq + ((l8 & 3) ^ (4 * (l8 >> 2))), vdst = 8 * lq + (l8 ^ (2 * lq));
+  const uint64_t once = policy_evict_first();
   int requested = 0;  // tiles whose keys were requested
   int page = -1, row = 0;
   auto fetch_page = [&]() {
@@ -351,7 +383,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
         for (int j = 0; j < 2 * KR; ++j, src += c.ks_token)
 #pragma unroll
           for (int y = 0; y < HC / 2; ++y)
-            cp_async_all(dst + 32 * (HC * (j % KR) + 2 * y) + (kdst ^ (4 * (j / KR))), src + 64 * y);
+            cp_async_once(dst + 32 * (HC * (j % KR) + 2 * y) + (kdst ^ (4 * (j / KR))), src + 64 * y, once);
       } else {
 #pragma unroll 1
         for (int j = 0; j < 2 * KR; ++j, src += c.ks_token)
@@ -359,6 +391,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
           for (int y = 0; y < HC / 2; ++y)
             cp_async_16(dst + 32 * (HC * (j % KR) + 2 * y) + (kdst ^ (4 * (j / KR))), j < left ? src + 64 * y : c.k,
                         j < left ? 16u : 0u);
+      }
+      if (asked != items) {  // the item's first tile here: its queries too, unless the place still waits for its reader
+        asked = items;
+        if (held <= used) {
+          held = items;
+          const int kvh = HT == 1 ? ri.h : ri.h / HT, head0 = kvh * G + (HT == 1 ? 0 : ri.h % HT) * 16;
+          const int rows = min(16, kvh * G + G - head0);
+          const uint16_t* qr = q + int64_t(ri.b) * sqb + int64_t(head0 + g) * sqh + 8 * t;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int h = 0; h < HC; ++h) {
+              const bool there = g + 8 * r < rows;
+              cp_async_16(ring + kUnits * (kUnit / 16) + (r * HC + h) * 32 + lane, there ? qr + 8 * r * sqh + 32 * h : q,
+                          there ? 16u : 0u);
+            }
+        }
       }
       ++requested;
       ++rtile;
@@ -389,7 +438,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
 #pragma unroll
         for (int j = 0; j < 2 * KR; ++j, src += c.vs_token)
 #pragma unroll
-          for (int v = 0; v < VC; ++v) cp_async_all(dst + 32 * (VC * j + v) + vdst, src + 64 * v);
+          for (int v = 0; v < VC; ++v) cp_async_once(dst + 32 * (VC * j + v) + vdst, src + 64 * v, once);
       } else {
 #pragma unroll 1
         for (int j = 0; j < 2 * KR; ++j, src += c.vs_token)
@@ -403,9 +452,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
   constexpr int kSlot = kUnit / 16;
   fetch_page();
   request_keys(ring);
-  request_values(ring + kSlot, 0);
+  request_values(ring + 2 * kSlot, 0);
   fetch_page();
-  request_keys(ring + 2 * kSlot);
+  request_keys(ring + kSlot);
+  request_values(ring + 3 * kSlot, 1);
+  fetch_page();
 
   const int prows = min(16, G), piece = piece_floats(prows, HD);
   // A negative scale turns the queries' signs instead, so that the largest product has the largest score.
@@ -413,20 +464,27 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
   const float scl = fabsf(scale_log2);
   uint32_t qb[R][2 * HC][2];
   float o[R][4 * VC][4], m[R][2], l[R][2];  // of heads 2t and 2t + 1 of each block of 8
-  int slot = 0, seg_tile0 = ctile;
+  int seg_tile0 = ctile;
   bool fresh = true, first_seg = true;  // of its run
   for (int n = 0;; ++n) {
+    // ---- scores
+    cp_async_wait<kUnits - 1>();
+    __syncwarp();
     if (fresh) {
       fresh = false;
       const int kvh = HT == 1 ? ci.h : ci.h / HT, head0 = kvh * G + (HT == 1 ? 0 : ci.h % HT) * 16;
       const int rows = min(16, kvh * G + G - head0);  // query heads of this item
       const uint16_t* qr = q + int64_t(ci.b) * sqb + int64_t(head0) * sqh + 8 * t;
+      const bool here = held == ++used;
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int h = 0; h < HC; ++h) {
           uint4 a = make_uint4(0u, 0u, 0u, 0u);
-          if (g + 8 * r < rows) a = __ldg(reinterpret_cast<const uint4*>(qr + int64_t(g + 8 * r) * sqh + 32 * h));
+          if (here)
+            a = ring[kUnits * kSlot + (r * HC + h) * 32 + lane];
+          else if (g + 8 * r < rows)
+            a = __ldg(reinterpret_cast<const uint4*>(qr + int64_t(g + 8 * r) * sqh + 32 * h));
           qb[r][2 * h][0] = a.x ^ flip, qb[r][2 * h][1] = a.y ^ flip;
           qb[r][2 * h + 1][0] = a.z ^ flip, qb[r][2 * h + 1][1] = a.w ^ flip;
         }
@@ -437,12 +495,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
         m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
       }
     }
-    // ---- scores
-    cp_async_wait<kUnits - 1>();
-    __syncwarp();
     float s[R][KI][4];  // rows g, g, g + 8, g + 8 of block i; heads 2t, 2t + 1, 2t, 2t + 1
     {
-      const uint4* src = ring + slot * kSlot;
+      const uint4* src = ring + (n & 1) * kSlot;
 #pragma unroll
       for (int i = 0; i < KI; ++i)
 #pragma unroll
@@ -459,9 +514,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
           }
         }
     }
-    request_values(ring + slot * kSlot, n + 1);
-    slot = slot == kUnits - 1 ? 0 : slot + 1;
-    fetch_page();
+    request_keys(ring + (n & 1) * kSlot);
     // ---- softmax; the lane's scores are those of its key rows KR * g + KI * e + i, entries [i][2 * e + head]
     const uint32_t f = flags >> ((n & 7) * 2);
     if (!(f & 1u)) {
@@ -552,7 +605,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
     cp_async_wait<kUnits - 1>();
     __syncwarp();
     {
-      const uint4* src = ring + slot * kSlot + 8 * t + (g ^ (2 * t));
+      const uint4* src = ring + (2 + (n & 1)) * kSlot + 8 * t + (g ^ (2 * t));
 #pragma unroll
       for (int v = 0; v < VC; ++v)
 #pragma unroll
@@ -570,8 +623,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_ctas(HD, TWO))
           }
         }
     }
-    request_keys(ring + slot * kSlot);
-    slot = slot == kUnits - 1 ? 0 : slot + 1;
+    request_values(ring + (2 + (n & 1)) * kSlot, n + 2);
+    fetch_page();
     // ---- end of the item, or of this run
     --cleft;
     if (ctile == ci.nt - 1 || cleft == 0) {
@@ -646,12 +699,11 @@ __global__ void __launch_bounds__(TPH == 32 ? 256 : TPH)
   constexpr int LX = HD / 4;                    // float4 columns
   constexpr int SL = TPH > LX ? TPH / LX : 1;   // slices over the pieces
   constexpr int CX = TPH > LX ? 1 : LX / TPH;   // columns per thread
-  constexpr int NW = TPH / 32;
   static_assert(CX == 1, "a warp covers a head's outputs");
   __shared__ float4 acc[TPH > 32 ? SL : 1][LX];
-  __shared__ float accl[TPH > 32 ? SL : 1], redm[NW];
+  __shared__ float2 accl[TPH > 32 ? SL : 1];
   const int64_t at = TPH == 32 ? int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  const int tid = threadIdx.x % TPH, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x % TPH;
   if (at >= int64_t(seqs) * nq) return;
   const int b = int(at / nq), head = int(at - int64_t(b) * nq);
   const int G = nq / kv_heads, kvh = head / G, ht = (head % G) / 16, row = (head % G) % 16, prows = min(16, G);
@@ -669,27 +721,18 @@ __global__ void __launch_bounds__(TPH == 32 ? 256 : TPH)
   const int first = 2 * r0 + (deal.first(r0) == t0 ? 0 : 1), pieces = r1 - r0 + 1;
   auto piece = [&](int i) { return partials + int64_t(i == 0 ? first : 2 * (r0 + i)) * piece_floats(prows, HD); };
   const int x = tid % LX, s = tid / LX;
-  float mx = -INFINITY;
-#pragma unroll 4
-  for (int i = tid; i < pieces; i += TPH) mx = fmaxf(mx, __ldcg(piece(i) + prows * HD + 2 * row));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-  if constexpr (TPH > 32) {
-    if (lane == 0) redm[tid >> 5] = mx;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NW; ++i) mx = fmaxf(mx, redm[i]);
-  }
-  const float base = mx == -INFINITY ? 0.0f : mx;
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float l = 0.0f;
+  float l = 0.0f, mx = -INFINITY;  // this thread's pieces, relative to their largest max
   constexpr int kBatch = 8;
   for (int i0 = s; i0 < pieces; i0 += kBatch * SL) {
     float2 e[kBatch];
     float4 v[kBatch];
+    float top = mx;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int i = i0 + k * SL;
+      e[k] = make_float2(-INFINITY, 0.0f);
+      v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (i < pieces) {
         const float* p = piece(i);
         e[k] = __ldcg(reinterpret_cast<const float2*>(p + prows * HD + 2 * row));
@@ -697,24 +740,34 @@ __global__ void __launch_bounds__(TPH == 32 ? 256 : TPH)
       }
     }
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      if (i0 + k * SL < pieces) {
-        const float f = ex2(e[k].x - base);
-        a.x = fmaf(v[k].x, f, a.x), a.y = fmaf(v[k].y, f, a.y), a.z = fmaf(v[k].z, f, a.z), a.w = fmaf(v[k].w, f, a.w);
-        l = fmaf(e[k].y, f, l);
-      }
+    for (int k = 0; k < kBatch; ++k) top = fmaxf(top, e[k].x);
+    const float base = top == -INFINITY ? 0.0f : top, g = ex2(mx - base);
+    a.x *= g, a.y *= g, a.z *= g, a.w *= g, l *= g;
+    mx = top;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float f = ex2(e[k].x - base);
+      a.x = fmaf(v[k].x, f, a.x), a.y = fmaf(v[k].y, f, a.y), a.z = fmaf(v[k].z, f, a.z), a.w = fmaf(v[k].w, f, a.w);
+      l = fmaf(e[k].y, f, l);
+    }
   }
   if constexpr (TPH > 32) {
     acc[s][x] = a;
-    if (x == 0) accl[s] = l;
+    if (x == 0) accl[s] = make_float2(mx, l);
     __syncthreads();
     if (s != 0) return;
-    for (int i = 1; i < SL; ++i) {
+    for (int i = 1; i < SL; ++i) mx = fmaxf(mx, accl[i].x);
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), l = 0.0f;
+    for (int i = 0; i < SL; ++i) {
       const float4 v = acc[i][x];
-      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-      l += accl[i];
+      const float f = ex2(accl[i].x - base);
+      a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
+      l = fmaf(accl[i].y, f, l);
     }
   } else if constexpr (SL == 2) {
+    const float top = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16)), f = ex2(mx - (top == -INFINITY ? 0.0f : top));
+    a.x *= f, a.y *= f, a.z *= f, a.w *= f, l *= f, mx = top;
     a.x += __shfl_xor_sync(0xFFFFFFFFu, a.x, 16), a.y += __shfl_xor_sync(0xFFFFFFFFu, a.y, 16);
     a.z += __shfl_xor_sync(0xFFFFFFFFu, a.z, 16), a.w += __shfl_xor_sync(0xFFFFFFFFu, a.w, 16);
     l += __shfl_xor_sync(0xFFFFFFFFu, l, 16);
@@ -902,10 +955,10 @@ template <bool F16, int HD, bool TWO, bool WEIGHTS>
 cudaError_t attn(const PagedCache& c, const PagedAttn& a, const PagedAttnWorkspace& w, int sms, cudaStream_t s) {
   const int HT = (a.nq / c.kv_heads + 15) / 16;
   auto kern = paged_attn_kernel<F16, HD, TWO, WEIGHTS>;
-  const size_t smem = size_t(kAttnWarps) * kUnits * kUnit + (2 * size_t(c.seqs) + 1) * 4;
+  const size_t smem = size_t(kAttnWarps) * attn_warp_smem(HD, TWO) + (2 * size_t(c.seqs) + 1) * 4;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  const int ctas = sms * attn_ctas(HD, TWO), workers = ctas * kAttnWarps;
+  const int ctas = sms * kAttnCtas, workers = ctas * kAttnWarps;
   if (w.counter && (e = cudaMemsetAsync(w.counter, 0, sizeof(int), s)) != cudaSuccess) return e;
   kern<<<ctas, kAttnWarps * 32, smem, s>>>(c, a.q, a.sqb, a.sqh, a.lens, a.out, a.nq, HT, a.scale * 1.4426950408889634f,
                                            w.partials, w.logits, w.logit_stride, w.ml, w.counter, w.starts);
@@ -942,7 +995,7 @@ void paged_set_page_size(PagedCache* c, int page_size) {
 size_t paged_attn_workspace(int seqs, int nq, int kv_heads, int head_dim, int capacity, bool weights, int sms,
                             void* base, PagedAttnWorkspace* w) {
   const int G = nq / kv_heads, tile = tile_of(head_dim), HT = (G + 15) / 16;
-  const int64_t workers = int64_t(sms) * attn_ctas(head_dim, G > 8) * kAttnWarps;
+  const int64_t workers = int64_t(sms) * kAttnCtas * kAttnWarps;
   const int64_t stride = (int64_t(capacity) + tile - 1) / tile * tile;
   // the lengths are on the device: runs are shared where the tables' whole capacity would call for it
   const bool shared = int64_t(seqs) * (stride / tile) * kv_heads * HT >= workers * kSharedFrom;
