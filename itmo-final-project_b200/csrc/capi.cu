@@ -683,7 +683,7 @@ int i4b_token_logprobs(const void* x, int dtype, int64_t rows, int64_t n, int64_
   DevInfo d;
   if (int st = current_device_info(&d)) return st;
   const cudaError_t e = launch_token_logprobs(x, dtype, rows, n, stride_x, targets, int(top), logprobs, entropy,
-                                              top_logprobs, top_ids, static_cast<cudaStream_t>(stream));
+                                              top_logprobs, top_ids, d.sms, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? I4B_OK : fail_cuda(e);
 }
 

@@ -224,6 +224,6 @@ cudaError_t launch_paged_evict(const PagedCache& c, const PagedEvict& e, cudaStr
 // logprobs.cu
 cudaError_t launch_token_logprobs(const void* x, int dtype, int64_t rows, int64_t n, int64_t stride,
                                   const int64_t* targets, int top, float* logprobs, float* entropy, float* top_lp,
-                                  int64_t* top_ids, cudaStream_t s);
+                                  int64_t* top_ids, int sms, cudaStream_t s);
 
 }  // namespace i4b

@@ -197,18 +197,22 @@ __device__ __forceinline__ int clamped_len(const PagedCache& c, const int32_t* l
 }
 
 // How `total` tiles are cut into runs.  The first `workers` runs are the warps' own: of `own` tiles, the first `longer`
-// of them of one more.  Where runs are shared, those of `more` tiles follow, and for the end ones of 2.
-constexpr int kSharedFrom = 16;  // tiles per warp from which on runs are shared
+// of them of one more.  Where runs are shared, those of `more` tiles follow, and for the end ones of `last`: 2 tiles
+// (16 KB), or as many as make a run 8 times its piece in the workspace.  Runs are shared from 8 `last` per warp on.
+__host__ __device__ constexpr int last_tiles(int rows, int head_dim) {
+  const int n = rows * head_dim * 4 * 8 / (2 * kUnit);
+  return n < 2 ? 2 : n;
+}
 
 struct Deal {
-  int total, workers, own, longer, more, long_end, more_end, more_runs;  // tiles: end of the own runs' longer ones, of ...
-  __device__ Deal(int total_, int workers_, bool shared) : total(total_), workers(workers_) {
+  int total, workers, last, own, longer, more, long_end, more_end, more_runs;  // tiles: end of the own runs' longer ones, of ...
+  __device__ Deal(int total_, int workers_, bool shared, int last_) : total(total_), workers(workers_), last(last_) {
     const int per = total / workers;
-    if (shared && per >= kSharedFrom) {
+    if (shared && per >= 8 * last) {
       own = per * 5 / 8;
       longer = 0;
-      more = max(4, per / 8);
-      more_runs = (total - workers * own - 2 * workers + more - 1) / more;  // (per - own >= 6; the last may end with the tiles)
+      more = max(2 * last, per / 8);
+      more_runs = (total - workers * own - last * workers + more - 1) / more;  // (the last may end with the tiles)
     } else {
       own = max(per, kMinTiles);
       longer = per >= kMinTiles ? total - workers * per : 0;
@@ -220,21 +224,21 @@ struct Deal {
   __device__ int64_t first(int r) const {
     if (r < workers) return int64_t(r) * own + min(r, longer);
     r -= workers;
-    return r < more_runs ? int64_t(workers) * own + longer + int64_t(r) * more : more_end + 2 * int64_t(r - more_runs);
+    return r < more_runs ? int64_t(workers) * own + longer + int64_t(r) * more : more_end + last * int64_t(r - more_runs);
   }
   __device__ int tiles(int r) const {
-    const int n = r < workers ? own + (r < longer ? 1 : 0) : (more == 0 ? 0 : (r < workers + more_runs ? more : 2));
+    const int n = r < workers ? own + (r < longer ? 1 : 0) : (more == 0 ? 0 : (r < workers + more_runs ? more : last));
     return int(min(int64_t(n), total - first(r)));
   }
   __device__ int run_of(int tile) const {
     if (tile < long_end) return tile / (own + 1);
     if (tile < int64_t(workers) * own + longer) return longer + (tile - long_end) / own;
     if (tile < more_end) return workers + (tile - workers * own - longer) / more;
-    return workers + more_runs + (tile - more_end) / 2;
+    return workers + more_runs + (tile - more_end) / last;
   }
 };
 
-// Runs per worker that a Deal makes at most: its own, (3/8 per + 2) / max(4, per / 8) < 4 and just over 1 of two tiles.
+// Runs per worker that a Deal makes at most: its own, (3/8 per + 2) / max(2 last, per / 8) < 4 and just over 1 at the end.
 constexpr int kMostRuns = 7;
 
 template <bool F16, int HD, bool TWO, bool WEIGHTS>
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
   if (blockIdx.x == 0)
     for (int b = tid; b <= B; b += kAttnWarps * 32) starts[b] = pre[b];  // for the join
   const int worker = int(blockIdx.x) * kAttnWarps + warp;
-  const Deal deal(pre[B], int(gridDim.x) * kAttnWarps, counter != nullptr);
+  const Deal deal(pre[B], int(gridDim.x) * kAttnWarps, counter != nullptr, last_tiles(min(16, G), HD));
 
   struct Item {
     int b, h, len, nt;  // sequence; kv head and tile of query heads; the sequence's length and tiles
@@ -709,7 +713,7 @@ __global__ void __launch_bounds__(TPH == 32 ? 256 : TPH)
   const int G = nq / kv_heads, kvh = head / G, ht = (head % G) / 16, row = (head % G) % 16, prows = min(16, G);
   pdl_wait();
   const int start = __ldcg(starts + b), nt = (__ldcg(starts + b + 1) - start) / (kv_heads * HT);
-  const Deal deal(__ldcg(starts + seqs), workers, shared != 0);
+  const Deal deal(__ldcg(starts + seqs), workers, shared != 0, last_tiles(prows, HD));
   uint16_t* dst = out + at * HD;
   if (nt == 0) {
     for (int i = tid; i < HD / 2; i += TPH) reinterpret_cast<uint32_t*>(dst)[i] = 0u;
@@ -998,7 +1002,8 @@ size_t paged_attn_workspace(int seqs, int nq, int kv_heads, int head_dim, int ca
   const int64_t workers = int64_t(sms) * kAttnCtas * kAttnWarps;
   const int64_t stride = (int64_t(capacity) + tile - 1) / tile * tile;
   // the lengths are on the device: runs are shared where the tables' whole capacity would call for it
-  const bool shared = int64_t(seqs) * (stride / tile) * kv_heads * HT >= workers * kSharedFrom;
+  const int last = last_tiles(std::min(G, 16), head_dim);
+  const bool shared = int64_t(seqs) * (stride / tile) * kv_heads * HT >= workers * 8 * last;
   const int64_t pieces = 2 * workers * (shared ? kMostRuns : 1);
   const size_t b0 = up256(size_t(pieces) * piece_floats(std::min(G, 16), head_dim) * 4), b1 = 256 + up256(4 * (size_t(seqs) + 1));
   const size_t b2 = weights ? up256(size_t(seqs) * nq * size_t(stride) * 4) : 0;
