@@ -342,7 +342,8 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
  * page_size rounded up] names the new pages, none of which may be a page that `cache` still reads in this call.
  * new_lens[seqs] = min(lens, budget); kept[seqs, kv_heads, budget] (contiguous) = the slots kept, -1 behind the last;
  * weights_out [seqs, kv_heads, width] = their weights, zeros behind the last (may be `weights` itself).
- * 0 <= recent <= budget, budget >= 1. */
+ * 0 <= recent <= budget, budget >= 1; max_pages * page_size <= I4B_EVICT_MAX_SLOTS. */
+#define I4B_EVICT_MAX_SLOTS 393216
 int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t stride_wb, int64_t stride_wh,
                     int64_t width, const int32_t* lens, const int32_t* new_table, int64_t new_table_stride,
                     int64_t new_max_pages, int64_t budget, int64_t recent, int32_t* new_lens, int32_t* kept,

@@ -657,7 +657,7 @@ int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t 
                     float* weights_out, int64_t stride_ob, int64_t stride_oh, void* stream) {
   PagedCache c;
   if (int st = paged_cache(cache, &c)) return st;
-  if (width < c.capacity || width > INT32_MAX - 64 || budget < 1 || budget > INT32_MAX - 64 || recent < 0 ||
+  if (c.capacity > paged_evict_most() || width < c.capacity || width > INT32_MAX - 64 || budget < 1 || budget > INT32_MAX - 64 || recent < 0 ||
       recent > budget || new_max_pages < (budget + c.page_size - 1) / c.page_size)
     return I4B_ERR_SHAPE;
   if (c.seqs == 0) return I4B_OK;
@@ -666,7 +666,7 @@ int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t 
   if (int st = current_device_info(&d)) return st;
   const PagedEvict p = {weights, stride_wb, stride_wh, lens, new_table, new_table_stride, int(budget), int(recent),
                         int(width), new_lens, kept, weights_out, stride_ob, stride_oh};
-  const cudaError_t e = launch_paged_evict(c, p, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_paged_evict(c, p, d.sms, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? I4B_OK : fail_cuda(e);
 }
 

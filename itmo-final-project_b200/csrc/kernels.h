@@ -219,7 +219,8 @@ cudaError_t launch_paged_attn(const PagedCache& c, const PagedAttn& a, const Pag
 cudaError_t launch_paged_append(const PagedCache& c, const uint16_t* qkv, int64_t sqkv, int64_t tokens, const void* cosT,
                                 const void* sinT, bool table32, int max_pos, const int32_t* positions,
                                 const int32_t* slots, const int32_t* seqs, uint16_t* q_out, int nq, cudaStream_t s);
-cudaError_t launch_paged_evict(const PagedCache& c, const PagedEvict& e, cudaStream_t s);
+int paged_evict_most();  // slots per sequence that eviction can select from
+cudaError_t launch_paged_evict(const PagedCache& c, const PagedEvict& e, int sms, cudaStream_t s);
 
 // logprobs.cu
 cudaError_t launch_token_logprobs(const void* x, int dtype, int64_t rows, int64_t n, int64_t stride,

@@ -820,121 +820,195 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kSelMost = 49152;  // slots of a row that one CTA of a cluster can hold
 
-// One CTA per (kv head, sequence): the order value of the `need`-th largest weight among the older positions by
-// radix selection (four passes over 8 bits), then the kept positions in order.
+__device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+// One cluster of `parts` CTAs per (kv head, sequence).  The row's weights lie in the CTAs' shared memory (read once,
+// so that the output may be the input); three histograms, of 11, 11 and 10 bits of the order value, each added up over
+// the cluster, give the `need`-th largest among the older positions; then every warp counts, and after one scan over
+// the warps of the cluster writes, what stays of its consecutive positions.
 __global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
     const float* weights, int64_t swb, int64_t swh, const int32_t* __restrict__ lens, int capacity, int budget,
     int recent, int32_t* __restrict__ new_lens, int32_t* __restrict__ kept, float* weights_out, int64_t sob,
-    int64_t soh, int width) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t found[2];
-  __shared__ uint32_t scan_tmp[32];
-  const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int64_t soh, int width, int kv_heads, int parts) {
+  extern __shared__ float row[];
+  __shared__ uint32_t hist[kBins], sum[kBins];
+  __shared__ uint32_t found[2], wcount[2][kSelWarps], total[2];
+  const int rank = parts > 1 ? int(cluster_ctarank()) : 0, item = int(blockIdx.x) / parts;
+  const int kvh = item % kv_heads, b = item / kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float* w = weights + b * swb + kvh * swh;
   float* wo = weights_out + b * sob + kvh * soh;
-  int32_t* ko = kept + (int64_t(b) * gridDim.x + kvh) * budget;
+  int32_t* ko = kept + int64_t(item) * budget;
   int L = __ldg(lens + b);
   L = L < 0 ? 0 : (L > capacity ? capacity : L);
   const int n = min(L, budget);
-  if (kvh == 0 && tid == 0) new_lens[b] = n;
-  const int old = L > budget ? L - recent : L;  // positions that compete
-  uint32_t thr = 0u;
-  uint32_t ties = 0u;  // how many of the positions at the threshold stay
-  if (L > budget) {
-    uint32_t need = uint32_t(budget - recent), mask = 0u;
-    for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0u;
+  if (item % kv_heads == 0 && rank == 0 && tid == 0) new_lens[b] = n;
+  const bool select = L > budget && budget > recent;
+  const int old = L > budget ? L - recent : L;  // positions that compete; all others stay
+  const int seg = (L + parts - 1) / parts, p0 = min(L, rank * seg), p1 = min(L, p0 + seg);
+  auto everyone = [&]() {
+    if (parts > 1)
+      cluster_sync();
+    else
       __syncthreads();
-      for (int i = tid; i < old; i += kSelThreads) {
-        const uint32_t u = order_of(w[i]);
-        if ((u & mask) == thr) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+  };
+
+  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
+  __syncthreads();
+#pragma unroll 8
+  for (int i = p0 + tid; i < p1; i += kSelThreads) {
+    const float v = w[i];
+    row[i - p0] = v;
+    if (select && i < old) atomicAdd(&hist[order_of(v) >> 21], 1u);
+  }
+  uint32_t thr = L > budget ? 0xFFFFFFFFu : 0u;  // (no weight has that order value: nothing but the recent ones stays)
+  uint32_t ties = 0u;                            // how many of the positions at the threshold stay
+  everyone();                                    // the whole row has been read
+  if (select) {
+    uint32_t need = uint32_t(budget - recent);
+    thr = 0u;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
+      if (pass > 0) {
+        const uint32_t mask = pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
+        for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
+        __syncthreads();
+        for (int i = p0 + tid; i < min(p1, old); i += kSelThreads) {
+          const uint32_t u = order_of(row[i - p0]);
+          if ((u & mask) == thr) atomicAdd(&hist[(u >> shift) & (bins - 1)], 1u);
+        }
+        everyone();
       }
+      // thread t owns bins 2t and 2t + 1 from the top; its count of the whole cluster, then a scan from the top
+      const int top = bins - 1 - 2 * tid;
+      uint32_t c0 = 0u, c1 = 0u;
+      if (top > 0) {
+        for (int r = 0; r < parts; ++r) {
+          c0 += parts > 1 ? ld_cluster_u32(&hist[top], uint32_t(r)) : hist[top];
+          c1 += parts > 1 ? ld_cluster_u32(&hist[top - 1], uint32_t(r)) : hist[top - 1];
+        }
+      }
+      uint32_t v = c0 + c1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (lane == 31) sum[warp] = v;
       __syncthreads();
-      if (tid == 0) {
-        uint32_t above = 0u;
-        int d = 255;
-        for (; d > 0 && above + hist[d] < need; --d) above += hist[d];
-        found[0] = uint32_t(d);
-        found[1] = above;
-      }
+      uint32_t above = v - c0 - c1;
+      for (int k = 0; k < warp; ++k) above += sum[k];
+      if (above < need && above + c0 >= need) found[0] = uint32_t(top), found[1] = above;
+      if (above + c0 < need && above + c0 + c1 >= need) found[0] = uint32_t(top - 1), found[1] = above + c0;
       __syncthreads();
       thr |= found[0] << shift;
       need -= found[1];
-      mask |= 255u << shift;
-      __syncthreads();
+      everyone();  // the histograms have been read
     }
     ties = need;
-    if (budget == recent) thr = 0xFFFFFFFFu;  // nothing of the older positions stays (no weight has this value)
   }
-  // kept positions in order: a scan over (ties before, kept before), both in one word pair
-  uint32_t tie_base = 0u, kept_base = 0u;
-  for (int i0 = 0; i0 < L; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    float v = 0.0f;
-    bool above = false, tie = false;
-    if (i < L) {
-      v = w[i];
-      const uint32_t u = order_of(v);
-      above = L <= budget || i >= old || u > thr;
-      tie = !above && u == thr && ties > 0u;
+  // each warp: consecutive positions, 32 at a time
+  const int per = ((p1 - p0 + kSelWarps - 1) / kSelWarps + 31) / 32 * 32, q0 = min(p1, p0 + warp * per), q1 = min(p1, q0 + per);
+  auto classify = [&](int i, uint32_t& above, uint32_t& tie) {
+    bool a = false, t = false;
+    if (i < q1) {
+      const uint32_t u = order_of(row[i - p0]);
+      a = L <= budget || i >= old || u > thr;
+      t = !a && ties > 0u && u == thr;
     }
-    const uint32_t bt = __ballot_sync(0xFFFFFFFFu, tie), below = (1u << lane) - 1u;
-    if (lane == 0) scan_tmp[warp] = __popc(bt);
-    __syncthreads();
-    uint32_t tb = tie_base, tall = 0u;
-    for (int k = 0; k < 32; ++k) {
-      if (k < warp) tb += scan_tmp[k];
-      tall += scan_tmp[k];
-    }
-    __syncthreads();
-    const bool keep = above || (tie && tb + __popc(bt & below) < ties);
-    const uint32_t bk = __ballot_sync(0xFFFFFFFFu, keep);
-    if (lane == 0) scan_tmp[warp] = __popc(bk);
-    __syncthreads();
-    uint32_t kb = kept_base, kall = 0u;
-    for (int k = 0; k < 32; ++k) {
-      if (k < warp) kb += scan_tmp[k];
-      kall += scan_tmp[k];
-    }
-    if (keep) {
-      const uint32_t at = kb + __popc(bk & below);
-      ko[at] = i;
-      wo[at] = v;  // at <= i: in place, this position's weight and all later ones are read by now
-    }
-    tie_base += tall;
-    kept_base += kall;
-    __syncthreads();
+    above = __ballot_sync(0xFFFFFFFFu, a);
+    tie = __ballot_sync(0xFFFFFFFFu, t);
+  };
+  uint32_t na = 0u, nt = 0u;
+  for (int i = q0; i < q1; i += 32) {
+    uint32_t a, t;
+    classify(i + lane, a, t);
+    na += __popc(a), nt += __popc(t);
   }
-  for (int i = n + tid; i < budget; i += kSelThreads) ko[i] = -1;
-  for (int i = n + tid; i < width; i += kSelThreads) wo[i] = 0.0f;
+  if (lane == 0) wcount[0][warp] = na, wcount[1][warp] = nt;
+  __syncthreads();
+  if (warp < 2) {  // exclusive scan over the CTA's warps, its sum for the cluster
+    const uint32_t own = wcount[warp][lane];
+    uint32_t v = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+      if (lane >= o) v += u;
+    }
+    wcount[warp][lane] = v - own;
+    if (lane == 31) total[warp] = v;
+  }
+  everyone();
+  uint32_t above = wcount[0][warp], tie = wcount[1][warp];
+  for (int r = 0; r < rank; ++r) above += ld_cluster_u32(&total[0], uint32_t(r)), tie += ld_cluster_u32(&total[1], uint32_t(r));
+  for (int i = q0; i < q1; i += 32) {
+    uint32_t a, t;
+    classify(i + lane, a, t);
+    const uint32_t below = (1u << lane) - 1u;
+    const uint32_t my_tie = tie + __popc(t & below);  // ties before this position
+    if ((a >> lane & 1u) || ((t >> lane & 1u) && my_tie < ties)) {
+      const uint32_t at = above + __popc(a & below) + min(my_tie, ties);
+      ko[at] = i + lane;
+      wo[at] = row[i + lane - p0];
+    }
+    above += __popc(a), tie += __popc(t);
+  }
+  for (int i = n + rank * kSelThreads + tid; i < budget; i += parts * kSelThreads) ko[i] = -1;
+  for (int i = n + rank * kSelThreads + tid; i < width; i += parts * kSelThreads) wo[i] = 0.0f;
+  if (parts > 1) cluster_sync();  // no CTA leaves while another may still read its shared memory
 }
 
-// Copies the kept rows into the new pages: a thread moves 16 bytes of keys and of values.
+// Copies the kept rows into the new pages: a thread moves 16 bytes of the keys and of the values of kCopyRows rows.
+constexpr int kCopyRows = 4;
 template <int HD>
 __global__ void __launch_bounds__(256) paged_evict_copy_kernel(const PagedCache c, const int32_t* __restrict__ kept,
                                                                const int32_t* __restrict__ new_table,
                                                                int64_t new_stride, int budget) {
-  constexpr int CH = HD / 8;
-  const int kvh = blockIdx.y, b = blockIdx.z;
-  const int i = (blockIdx.x * 256 + threadIdx.x) / CH, ch = threadIdx.x % CH;
+  constexpr int CH = HD / 8, ROWS = 256 / CH;
+  const int kvh = blockIdx.y, b = blockIdx.z, ch = threadIdx.x % CH;
+  const int i0 = blockIdx.x * (ROWS * kCopyRows) + threadIdx.x / CH;
+  const int32_t* table = c.table + int64_t(b) * c.table_stride;
   pdl_wait();
-  if (i >= budget) return;
-  const int pos = __ldcg(kept + (int64_t(b) * c.kv_heads + kvh) * budget + i);
-  if (pos < 0) return;
-  const int pi = page_of(c, pos), po = page_of(c, i);
-  const int from = page_entry(c, c.table + int64_t(b) * c.table_stride, pi);
-  const int to = page_entry(c, new_table + int64_t(b) * new_stride, po);
-  if (to < 0) return;
-  const int64_t r = pos - pi * c.page_size, ro = i - po * c.page_size;
-  uint4 kk = make_uint4(0u, 0u, 0u, 0u), vv = kk;
-  if (from >= 0) {
-    kk = *reinterpret_cast<const uint4*>(c.k + from * c.ks_page + kvh * c.ks_head + r * c.ks_token + 8 * ch);
-    vv = *reinterpret_cast<const uint4*>(c.v + from * c.vs_page + kvh * c.vs_head + r * c.vs_token + 8 * ch);
+  int pos[kCopyRows];
+#pragma unroll
+  for (int k = 0; k < kCopyRows; ++k) {
+    const int i = i0 + k * ROWS;
+    pos[k] = i < budget ? __ldcg(kept + (int64_t(b) * c.kv_heads + kvh) * budget + i) : -1;
   }
-  *reinterpret_cast<uint4*>(c.k + to * c.ks_page + kvh * c.ks_head + ro * c.ks_token + 8 * ch) = kk;
-  *reinterpret_cast<uint4*>(c.v + to * c.vs_page + kvh * c.vs_head + ro * c.vs_token + 8 * ch) = vv;
+  int from[kCopyRows], to[kCopyRows];
+#pragma unroll
+  for (int k = 0; k < kCopyRows; ++k) {
+    from[k] = to[k] = -1;
+    if (pos[k] >= 0) {
+      from[k] = page_entry(c, table, page_of(c, pos[k]));
+      to[k] = page_entry(c, new_table + int64_t(b) * new_stride, page_of(c, i0 + k * ROWS));
+    }
+  }
+  uint4 kk[kCopyRows], vv[kCopyRows];
+#pragma unroll
+  for (int k = 0; k < kCopyRows; ++k) {
+    kk[k] = vv[k] = make_uint4(0u, 0u, 0u, 0u);  // (a page that holds nothing)
+    if (from[k] >= 0) {
+      const int r = pos[k] - page_of(c, pos[k]) * c.page_size;
+      kk[k] = __ldcs(reinterpret_cast<const uint4*>(c.k + from[k] * c.ks_page + kvh * c.ks_head + int64_t(r) * c.ks_token + 8 * ch));
+      vv[k] = __ldcs(reinterpret_cast<const uint4*>(c.v + from[k] * c.vs_page + kvh * c.vs_head + int64_t(r) * c.vs_token + 8 * ch));
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kCopyRows; ++k) {
+    if (to[k] < 0) continue;
+    const int i = i0 + k * ROWS, r = i - page_of(c, i) * c.page_size;
+    *reinterpret_cast<uint4*>(c.k + to[k] * c.ks_page + kvh * c.ks_head + int64_t(r) * c.ks_token + 8 * ch) = kk[k];
+    *reinterpret_cast<uint4*>(c.v + to[k] * c.vs_page + kvh * c.vs_head + int64_t(r) * c.vs_token + 8 * ch) = vv[k];
+  }
 }
 
 // Launch that may start while its predecessor drains; the kernel waits (griddepcontrol.wait) before reading.
@@ -1047,14 +1121,35 @@ cudaError_t launch_paged_append(const PagedCache& c, const uint16_t* qkv, int64_
   return cudaGetLastError();
 }
 
-cudaError_t launch_paged_evict(const PagedCache& c, const PagedEvict& e, cudaStream_t s) {
-  paged_evict_select_kernel<<<dim3(unsigned(c.kv_heads), unsigned(c.seqs)), kSelThreads, 0, s>>>(
-      e.weights, e.swb, e.swh, e.lens, std::min(c.capacity, e.width), e.budget, e.recent, e.new_lens, e.kept,
-      e.weights_out, e.sob, e.soh, e.width);
-  cudaError_t st = cudaGetLastError();
+int paged_evict_most() { return 8 * kSelMost; }
+
+cudaError_t launch_paged_evict(const PagedCache& c, const PagedEvict& e, int sms, cudaStream_t s) {
+  // CTAs per row: as many as hold it at 64 KB each (two per SM), more while the SMs are not all busy and each still has
+  // two positions per thread; rows beyond 8 x 64 KB take up to 192 KB each
+  const int rows = c.seqs * c.kv_heads;
+  int parts = 1;
+  while (parts < 8 && c.capacity > parts * 16384) parts *= 2;
+  while (parts < 8 && rows * parts * 2 <= sms && c.capacity > parts * 4096) parts *= 2;
+  const size_t smem = size_t((c.capacity + parts - 1) / parts + 1) * 4;
+  cudaError_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(paged_evict_select_kernel), smem);
   if (st != cudaSuccess) return st;
-  const int rows = 256 / (c.head_dim / 8);
-  const dim3 grid(unsigned((e.budget + rows - 1) / rows), unsigned(c.kv_heads), unsigned(c.seqs));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(rows * parts));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(parts);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  st = cudaLaunchKernelEx(&cfg, paged_evict_select_kernel, e.weights, e.swb, e.swh, e.lens, c.capacity, e.budget, e.recent,
+                          e.new_lens, e.kept, e.weights_out, e.sob, e.soh, e.width, c.kv_heads, parts);
+  if (st != cudaSuccess) return st;
+  const int per = 256 / (c.head_dim / 8) * kCopyRows;
+  const dim3 grid(unsigned((e.budget + per - 1) / per), unsigned(c.kv_heads), unsigned(c.seqs));
   if (c.head_dim == 64)
     return launch_after(paged_evict_copy_kernel<64>, grid, dim3(256), 0, s, c, static_cast<const int32_t*>(e.kept),
                         e.new_table, e.new_stride, e.budget);

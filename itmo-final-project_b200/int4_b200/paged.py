@@ -21,6 +21,7 @@ import torch
 from . import _lib
 
 _HALF = (torch.bfloat16, torch.float16)
+EVICT_MAX_SLOTS = 393216  # I4B_EVICT_MAX_SLOTS
 
 
 def _need(ok: bool, what: str) -> None:
@@ -173,6 +174,7 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
     _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
           and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1),
           f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
+    _need(width * page <= EVICT_MAX_SLOTS, f"{width * page} slots per sequence: eviction selects from at most {EVICT_MAX_SLOTS}")
     _indices(lens, "lens", B)
     _table(new_table, "new_table")
     _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget} and recent {recent}: 0 <= recent <= budget, budget >= 1")
