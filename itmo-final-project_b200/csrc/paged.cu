@@ -813,17 +813,32 @@ __global__ void __launch_bounds__(256) paged_attn_weights_kernel(const PagedCach
 // ------------------------------------------------------------------ eviction
 
 // Weights as unsigned integers in the order of their values: NaN lowest, then -inf, ..., -0 = +0, ..., +inf.
-__device__ __forceinline__ uint32_t order_of(float w) {
-  if (w != w) return 0u;
-  if (w == 0.0f) return 0x80000000u;
-  const uint32_t u = __float_as_uint(w);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+__device__ __forceinline__ uint32_t order_of(uint32_t u) {
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
+  return u & 0x80000000u ? (u == 0x80000000u ? u : ~u) : u | 0x80000000u;
+}
+// Of four at once; +0 to +inf, what accumulated weights are, take the short way.
+__device__ __forceinline__ uint4 order_of(const uint4& w) {
+  if (max(max(w.x, w.y), max(w.z, w.w)) <= 0x7F800000u)
+    return make_uint4(w.x | 0x80000000u, w.y | 0x80000000u, w.z | 0x80000000u, w.w | 0x80000000u);
+  return make_uint4(order_of(w.x), order_of(w.y), order_of(w.z), order_of(w.w));
 }
 
 constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kSelMost = 49152;  // slots of a row that one CTA of a cluster can hold
 
+// hist[i] += 1 in shared memory where `yes`: predicated, a branch around each would cost more than the addition.
+__device__ __forceinline__ void count_if(uint32_t* hist, uint32_t i, bool yes) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p red.shared.add.u32 [%0], 1;\n\t}" ::"r"(smem_u32(hist + i)),
+               "r"(uint32_t(yes))
+               : "memory");
+}
+__device__ __forceinline__ uint2 ld_cluster_u64(const uint32_t* p, uint32_t rank) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t rank) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
@@ -834,12 +849,13 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t r
 // so that the output may be the input); three histograms, of 11, 11 and 10 bits of the order value, each added up over
 // the cluster, give the `need`-th largest among the older positions; then every warp counts, and after one scan over
 // the warps of the cluster writes, what stays of its consecutive positions.
-__global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
+__global__ void __launch_bounds__(kSelThreads, 2) paged_evict_select_kernel(
     const float* weights, int64_t swb, int64_t swh, const int32_t* __restrict__ lens, int capacity, int budget,
     int recent, int32_t* __restrict__ new_lens, int32_t* __restrict__ kept, float* weights_out, int64_t sob,
     int64_t soh, int width, int kv_heads, int parts) {
-  extern __shared__ float row[];
-  __shared__ uint32_t hist[kBins], sum[kBins];
+  extern __shared__ __align__(16) uint32_t row[];
+  __shared__ __align__(8) uint32_t hist[kBins];
+  __shared__ uint32_t sum[kSelWarps];
   __shared__ uint32_t found[2], wcount[2][kSelWarps], total[2];
   const int rank = parts > 1 ? int(cluster_ctarank()) : 0, item = int(blockIdx.x) / parts;
   const int kvh = item % kv_heads, b = item / kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -852,7 +868,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
   if (item % kv_heads == 0 && rank == 0 && tid == 0) new_lens[b] = n;
   const bool select = L > budget && budget > recent;
   const int old = L > budget ? L - recent : L;  // positions that compete; all others stay
-  const int seg = (L + parts - 1) / parts, p0 = min(L, rank * seg), p1 = min(L, p0 + seg);
+  const int seg = ((L + parts - 1) / parts + 3) / 4 * 4, p0 = min(L, rank * seg), p1 = min(L, p0 + seg), np = p1 - p0;
+  const int rival = min(np, max(0, old - p0));  // of this CTA's positions, those that compete
   auto everyone = [&]() {
     if (parts > 1)
       cluster_sync();
@@ -862,11 +879,31 @@ __global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
 
   for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
   __syncthreads();
-#pragma unroll 8
-  for (int i = p0 + tid; i < p1; i += kSelThreads) {
-    const float v = w[i];
-    row[i - p0] = v;
-    if (select && i < old) atomicAdd(&hist[order_of(v) >> 21], 1u);
+  auto count4 = [&](int i, const uint4& k, uint32_t mask, uint32_t want, int shift, uint32_t low) {
+    const uint32_t e[4] = {k.x, k.y, k.z, k.w};
+    if (i + 4 <= rival) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) count_if(hist, (e[u] >> shift) & low, (e[u] & mask) == want);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) count_if(hist, (e[u] >> shift) & low, (e[u] & mask) == want && i + u < rival);
+    }
+  };
+  const bool vec = (reinterpret_cast<uintptr_t>(w + p0) & 15) == 0;
+#pragma unroll 4
+  for (int i = 4 * tid; i < np; i += 4 * kSelThreads) {
+    uint4 v;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(w + p0 + i);
+    if (vec && i + 4 <= np) {
+      v = *reinterpret_cast<const uint4*>(src);
+    } else {
+      v.x = src[0];
+      v.y = i + 1 < np ? src[1] : 0u;
+      v.z = i + 2 < np ? src[2] : 0u;
+      v.w = i + 3 < np ? src[3] : 0u;
+    }
+    *reinterpret_cast<uint4*>(row + i) = v;
+    if (select) count4(i, order_of(v), 0u, 0u, 21, 2047u);
   }
   uint32_t thr = L > budget ? 0xFFFFFFFFu : 0u;  // (no weight has that order value: nothing but the recent ones stays)
   uint32_t ties = 0u;                            // how many of the positions at the threshold stay
@@ -881,10 +918,9 @@ __global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
         const uint32_t mask = pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
         for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
         __syncthreads();
-        for (int i = p0 + tid; i < min(p1, old); i += kSelThreads) {
-          const uint32_t u = order_of(row[i - p0]);
-          if ((u & mask) == thr) atomicAdd(&hist[(u >> shift) & (bins - 1)], 1u);
-        }
+#pragma unroll 4
+        for (int i = 4 * tid; i < rival; i += 4 * kSelThreads)
+          count4(i, order_of(*reinterpret_cast<const uint4*>(row + i)), mask, thr, shift, uint32_t(bins - 1));
         everyone();
       }
       // thread t owns bins 2t and 2t + 1 from the top; its count of the whole cluster, then a scan from the top
@@ -892,8 +928,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
       uint32_t c0 = 0u, c1 = 0u;
       if (top > 0) {
         for (int r = 0; r < parts; ++r) {
-          c0 += parts > 1 ? ld_cluster_u32(&hist[top], uint32_t(r)) : hist[top];
-          c1 += parts > 1 ? ld_cluster_u32(&hist[top - 1], uint32_t(r)) : hist[top - 1];
+          const uint2 c = parts > 1 ? ld_cluster_u64(&hist[top - 1], uint32_t(r)) : *reinterpret_cast<const uint2*>(&hist[top - 1]);
+          c0 += c.y, c1 += c.x;
         }
       }
       uint32_t v = c0 + c1;
@@ -904,8 +940,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
       }
       if (lane == 31) sum[warp] = v;
       __syncthreads();
-      uint32_t above = v - c0 - c1;
-      for (int k = 0; k < warp; ++k) above += sum[k];
+      const uint32_t above = v - c0 - c1 + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? sum[lane] : 0u);
       if (above < need && above + c0 >= need) found[0] = uint32_t(top), found[1] = above;
       if (above + c0 < need && above + c0 + c1 >= need) found[0] = uint32_t(top - 1), found[1] = above + c0;
       __syncthreads();
@@ -915,24 +950,35 @@ __global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
     }
     ties = need;
   }
-  // each warp: consecutive positions, 32 at a time
-  const int per = ((p1 - p0 + kSelWarps - 1) / kSelWarps + 31) / 32 * 32, q0 = min(p1, p0 + warp * per), q1 = min(p1, q0 + per);
-  auto classify = [&](int i, uint32_t& above, uint32_t& tie) {
-    bool a = false, t = false;
+  // each warp: consecutive positions, 128 at a time, four per lane; what stays as bits 0-3 (above the threshold, or not
+  // competing) and 4-7 (at it)
+  const int per = ((np + kSelWarps - 1) / kSelWarps + 127) / 128 * 128, q0 = min(np, warp * per), q1 = min(np, q0 + per);
+  auto classify = [&](int i, uint4& v) {
+    uint32_t m = 0u;
     if (i < q1) {
-      const uint32_t u = order_of(row[i - p0]);
-      a = L <= budget || i >= old || u > thr;
-      t = !a && ties > 0u && u == thr;
+      v = *reinterpret_cast<const uint4*>(row + i);
+      const uint4 k = order_of(v);
+      const uint32_t e[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) m |= (e[u] > thr ? 1u << u : 0u) | (e[u] == thr ? 16u << u : 0u);
+      if (L <= budget) m = 15u;
+      if (i + 4 > rival) {  // some of them do not compete, or are not there
+        const uint32_t stay = i >= rival ? 15u : (15u << (rival - i)) & 15u;
+        m = (m & ~(stay | stay << 4)) | stay;
+      }
+      if (i + 4 > np) m &= ((1u << (np - i)) - 1u) * 17u;
     }
-    above = __ballot_sync(0xFFFFFFFFu, a);
-    tie = __ballot_sync(0xFFFFFFFFu, t);
+    return m;
   };
-  uint32_t na = 0u, nt = 0u;
-  for (int i = q0; i < q1; i += 32) {
-    uint32_t a, t;
-    classify(i + lane, a, t);
-    na += __popc(a), nt += __popc(t);
+  uint32_t na = 0u, nt = 0u, known = 0u;  // the first four answers are kept
+#pragma unroll 4
+  for (int i = q0 + 4 * lane, k = 0; i - 4 * lane < q1; i += 128, k += 8) {
+    uint4 v;
+    const uint32_t m = classify(i, v);
+    if (k < 32) known |= m << k;
+    na += __popc(m & 15u), nt += __popc(m >> 4);
   }
+  na = __reduce_add_sync(0xFFFFFFFFu, na), nt = __reduce_add_sync(0xFFFFFFFFu, nt);
   if (lane == 0) wcount[0][warp] = na, wcount[1][warp] = nt;
   __syncthreads();
   if (warp < 2) {  // exclusive scan over the CTA's warps, its sum for the cluster
@@ -949,20 +995,46 @@ __global__ void __launch_bounds__(kSelThreads) paged_evict_select_kernel(
   everyone();
   uint32_t above = wcount[0][warp], tie = wcount[1][warp];
   for (int r = 0; r < rank; ++r) above += ld_cluster_u32(&total[0], uint32_t(r)), tie += ld_cluster_u32(&total[1], uint32_t(r));
-  for (int i = q0; i < q1; i += 32) {
-    uint32_t a, t;
-    classify(i + lane, a, t);
-    const uint32_t below = (1u << lane) - 1u;
-    const uint32_t my_tie = tie + __popc(t & below);  // ties before this position
-    if ((a >> lane & 1u) || ((t >> lane & 1u) && my_tie < ties)) {
-      const uint32_t at = above + __popc(a & below) + min(my_tie, ties);
-      ko[at] = i + lane;
-      wo[at] = row[i + lane - p0];
+#pragma unroll 1
+  for (int i = q0 + 4 * lane, k = 0; i - 4 * lane < q1; i += 128, k += 8) {
+    uint4 v;
+    const uint32_t m = k < 32 ? known >> k & 255u : classify(i, v);
+    if (__ballot_sync(0xFFFFFFFFu, m != 0u) == 0u) continue;
+    const uint32_t own = __popc(m & 15u) | __popc(m >> 4) << 16;
+    uint32_t scan = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, scan, o);
+      if (lane >= o) scan += u;
     }
-    above += __popc(a), tie += __popc(t);
+    const uint32_t all = __shfl_sync(0xFFFFFFFFu, scan, 31);
+    uint32_t a = above + ((scan - own) & 0xFFFFu), t = tie + ((scan - own) >> 16);  // before this lane's positions
+    if (m) {
+      v = *reinterpret_cast<const uint4*>(row + i);
+      const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool is_a = m >> u & 1u, is_t = m >> (4 + u) & 1u;
+        if (is_a || (is_t && t < ties)) {
+          const uint32_t at = a + min(t, ties);
+          ko[at] = p0 + i + u;
+          wo[at] = __uint_as_float(e[u]);
+        }
+        a += is_a, t += is_t;
+      }
+    }
+    above += all & 0xFFFFu, tie += all >> 16;
   }
   for (int i = n + rank * kSelThreads + tid; i < budget; i += parts * kSelThreads) ko[i] = -1;
-  for (int i = n + rank * kSelThreads + tid; i < width; i += parts * kSelThreads) wo[i] = 0.0f;
+  if ((reinterpret_cast<uintptr_t>(wo) & 15) == 0) {
+    const int n4 = (n + 3) / 4 * 4, w4 = width / 4 * 4;
+    for (int i = n4 + 4 * (rank * kSelThreads + tid); i < w4; i += 4 * parts * kSelThreads)
+      *reinterpret_cast<float4*>(wo + i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (rank == 0 && tid < 4 && n + tid < min(n4, width)) wo[n + tid] = 0.0f;
+    if (rank == 0 && tid < 4 && w4 >= n4 && w4 + tid < width) wo[w4 + tid] = 0.0f;
+  } else {
+    for (int i = n + rank * kSelThreads + tid; i < width; i += parts * kSelThreads) wo[i] = 0.0f;
+  }
   if (parts > 1) cluster_sync();  // no CTA leaves while another may still read its shared memory
 }
 
@@ -1130,7 +1202,7 @@ cudaError_t launch_paged_evict(const PagedCache& c, const PagedEvict& e, int sms
   int parts = 1;
   while (parts < 8 && c.capacity > parts * 16384) parts *= 2;
   while (parts < 8 && rows * parts * 2 <= sms && c.capacity > parts * 4096) parts *= 2;
-  const size_t smem = size_t((c.capacity + parts - 1) / parts + 1) * 4;
+  const size_t smem = size_t((c.capacity + parts - 1) / parts + 4) * 4;
   cudaError_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(paged_evict_select_kernel), smem);
   if (st != cudaSuccess) return st;
   cudaLaunchConfig_t cfg = {};
