@@ -34,10 +34,10 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0):
     if V > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < 0:
         x = x.contiguous()
     targets = targets.contiguous()
-    lp = torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    top_lp = torch.empty((*lead, top), dtype=torch.float32, device=dev) if top else None
-    top_ids = torch.empty((*lead, top), dtype=torch.int64, device=dev) if top else None
+    lp = torch.empty_like(targets, dtype=torch.float32)
+    entropy = torch.empty_like(lp)
+    top_lp = lp.new_empty((*lead, top)) if top else None
+    top_ids = targets.new_empty((*lead, top)) if top else None
     with _lib.on_device(dev):
         st = _lib.lib().i4b_token_logprobs(x.data_ptr(), _lib.DTYPE_CODE[x.dtype], x.shape[0], V, x.stride(0),
                                            targets.data_ptr(), top, lp.data_ptr(), entropy.data_ptr(),

@@ -16,6 +16,8 @@ reference, whose decode benchmark uses transformers' StaticCache (``benchmarks/e
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -27,6 +29,13 @@ EVICT_MAX_SLOTS = 393216  # I4B_EVICT_MAX_SLOTS
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(B: int, nq: int, nkv: int, dim: int, capacity: int, weights: bool, device: int) -> int:
+    """Bytes of workspace: a matter of the sizes (and of the device's SMs) alone."""
+    with torch.cuda.device(device):
+        return _lib.lib().i4b_paged_attention_workspace_size(B, nq, nkv, dim, capacity, weights)
 
 
 def _on_gpu(device: torch.device, *tensors) -> None:
@@ -96,7 +105,7 @@ def paged_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos
     else:
         _need(T <= block_table.shape[0], f"{T} tokens without seqs, and a block table of {block_table.shape[0]} sequences")
     if out is None:
-        out = torch.empty((T, nq, dim), dtype=qkv.dtype, device=qkv.device)
+        out = qkv.new_empty((T, nq, dim))
     else:
         _need(out.shape == (T, nq, dim) and out.dtype == qkv.dtype and out.is_contiguous(),
               "out must be a contiguous [tokens, nq, head_dim] of the caches' dtype")
@@ -142,12 +151,11 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     dev = q.device
     _on_gpu(dev, k_cache, v_cache, block_table, lens, weights, out)
     q = _rows16(q)
-    L = _lib.lib()
+    need = _attention_workspace(B, nq, nkv, dim, width * page, weights is not None, dev.index)
+    # from torch's allocator each time: two captured graphs never share it, and eager streams do not either
+    ws = lens.new_empty(need, dtype=torch.uint8)
     with _lib.on_device(dev):
-        need = L.i4b_paged_attention_workspace_size(B, nq, nkv, dim, width * page, weights is not None)
-        # from torch's allocator each time: two captured graphs never share it, and eager streams do not either
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        st = L.i4b_paged_decode_attention(c, q.data_ptr(), q.stride(0), q.stride(1), nq, lens.data_ptr(),
+        st = _lib.lib().i4b_paged_decode_attention(c, q.data_ptr(), q.stride(0), q.stride(1), nq, lens.data_ptr(),
                                           dim ** -0.5 if scale is None else scale, out.data_ptr(),
                                           None if weights is None else weights.data_ptr(),
                                           0 if weights is None else weights.stride(0),
@@ -182,13 +190,13 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
           f"new_table must hold {-(-budget // page)} pages for each of {B} sequences")
     dev = weights.device
     if weights_out is None:
-        weights_out = torch.empty(weights.shape, dtype=torch.float32, device=dev)
+        weights_out = torch.empty_like(weights, memory_format=torch.contiguous_format)
     else:
         _need(weights_out.shape == weights.shape and weights_out.dtype == torch.float32
               and (weights.shape[2] <= 1 or weights_out.stride(2) == 1), "weights_out must be float32 of the weights' shape")
     _on_gpu(dev, k_cache, v_cache, block_table, lens, new_table, weights_out)
-    new_lens = torch.empty(B, dtype=torch.int32, device=dev)
-    kept = torch.empty((B, nkv, budget), dtype=torch.int32, device=dev)
+    new_lens = torch.empty_like(lens)
+    kept = lens.new_empty((B, nkv, budget))
     with _lib.on_device(dev):
         st = _lib.lib().i4b_paged_evict(c, weights.data_ptr(), weights.stride(0), weights.stride(1),
                                         weights.shape[2], lens.data_ptr(), new_table.data_ptr(), new_table.stride(0),
