@@ -19,7 +19,6 @@ namespace i4b {
 
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kCand = 512;  // candidates above, and at, the threshold that a CTA holds
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -183,6 +182,7 @@ __device__ __forceinline__ void add_batch(Stat& st, const uint4 (&w)[N]) {
 // Whether (v, i) comes before (w, j) among the most probable tokens: larger value, then lower index; never for a NaN.
 __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
+template <int kThreads>
 struct Shared {
   Stat red[kThreads / 32], part;
   float col[kThreads / 32][32];
@@ -196,14 +196,16 @@ struct Shared {
   int si[I4B_MAX_TOP];
 };
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 2)
+// kThreads: 512 for few rows, 256 (four CTAs per SM, whose beginnings and ends overlap) when there are rows for all
+// SMs: 96 against 88 us for 2048 x 128256 bf16.
+template <int DT, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     token_logprobs_kernel(const typename Logit<DT>::T* __restrict__ x, int n, int64_t stride,
                           const int64_t* __restrict__ targets, int top, int parts, float* __restrict__ logprobs,
                           float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_ids) {
   using E = Logit<DT>;
   constexpr int VEC = E::kVec, U = 4;
-  __shared__ Shared sh;
+  __shared__ Shared<kThreads> sh;
   const int64_t row = blockIdx.x / parts;
   const int part = parts > 1 ? int(cluster_ctarank()) : 0;
   const typename E::T* xr = x + row * stride;
@@ -430,9 +432,10 @@ cudaError_t launch(const void* x, int64_t rows, int64_t n, int64_t stride, const
   // as many CTAs per row as keep all CTAs resident (two per SM), each with at least 16 KB
   int parts = 8;
   while (parts > 1 && (rows * parts > 2 * sms || n * int64_t(sizeof(T)) < parts * 16384)) parts /= 2;
+  const bool many = rows >= 2 * sms;  // (parts is 1)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(rows * parts));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(many ? 256 : 512);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -441,8 +444,9 @@ cudaError_t launch(const void* x, int64_t rows, int64_t n, int64_t stride, const
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = parts > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DT>, static_cast<const T*>(x), int(n), stride, targets, top, parts,
-                            logprobs, entropy, top_lp, top_ids);
+  return cudaLaunchKernelEx(&cfg, many ? token_logprobs_kernel<DT, 256> : token_logprobs_kernel<DT, 512>,
+                            static_cast<const T*>(x), int(n), stride, targets, top, parts, logprobs, entropy, top_lp,
+                            top_ids);
 }
 
 }  // namespace
