@@ -612,9 +612,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
             }
           }
     }
-    // probabilities; rounded to the values' type for the second product (half a step each, as the output is),
-    // summed unrounded
-    uint32_t pb[R][KI][2];
+    // probabilities, for the second product as the sum of two values of the cache's type (the rounded one and what that
+    // leaves): rounded once, they would be off as much as the output's own rounding is
+    uint32_t pb[R][KI][2], pc[R][KI][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float n0 = m[r][0] == -INFINITY ? 0.0f : -m[r][0], n1 = m[r][1] == -INFINITY ? 0.0f : -m[r][1];
@@ -629,7 +629,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
             p1 = x1 == -INFINITY ? 0.0f : p1;
           }
           l[r][0] += p0, l[r][1] += p1;
-          pb[r][i][e] = transpose8(pack2<F16>(p0, p1));
+          const uint32_t w = pack2<F16>(p0, p1);
+          const float2 back = unpack2<F16>(w);
+          pb[r][i][e] = transpose8(w);
+          pc[r][i][e] = transpose8(pack2<F16>(p0 - back.x, p1 - back.y));
         }
     }
     // ---- output: dims 8(g + 8v) + 2w and + 2w + 1 are rows g and g + 8 of block 4v + w
@@ -650,7 +653,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
             const uint32_t va[4] = {__byte_perm(x0[w], y0[w], 0x5410), __byte_perm(x0[w], y0[w], 0x7632),
                                     __byte_perm(x1[w], y1[w], 0x5410), __byte_perm(x1[w], y1[w], 0x7632)};
 #pragma unroll
-            for (int r = 0; r < R; ++r) mma_16816<F16>(o[r][4 * v + w], va, pb[r][i][0], pb[r][i][1]);
+            for (int r = 0; r < R; ++r) {
+              mma_16816<F16>(o[r][4 * v + w], va, pb[r][i][0], pb[r][i][1]);
+              mma_16816<F16>(o[r][4 * v + w], va, pc[r][i][0], pc[r][i][1]);
+            }
           }
         }
     }
