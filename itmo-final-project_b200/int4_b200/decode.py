@@ -20,6 +20,10 @@ the projections laid out for the kernels and for tensor parallelism:
   tables rounded to bf16, scaled-dot-product attention), so a one-rank
   ``LlamaTP`` matches the HF model with the same weights.
 
+``paged_cache`` / ``prefill_paged`` / ``decode_paged`` run the same model over a
+paged key-value cache, for sequences of different lengths (``paged``), and
+``score`` returns the log probabilities of given tokens (``logprobs``).
+
 ``w4=False`` keeps every projection in bf16 (``torch.nn.functional.linear``):
 the same model and decode loop, for the W4-versus-bf16 comparison.  All
 steps are free of host synchronisation and of shape changes, so a decode
@@ -34,6 +38,8 @@ import torch.nn.functional as F
 
 from . import _lib
 from .gemm import w4a16_matmul, w4a16_matmul_argmax
+from .logprobs import token_logprobs
+from .paged import PagedKVCache, paged_decode_attention, paged_kv_append
 from .peer import argmax_allreduce, w4a16_matmul_allreduce
 from .quantize import quantize_int4
 
@@ -578,19 +584,104 @@ class LlamaTP:
         assert self.fused, "the unfused decode step has no separate hidden-state form"
         return self._decode_step_fused(ids, pos)
 
+    @torch.no_grad()
+    def score(self, ids: torch.Tensor, top: int = 0):
+        """Log probabilities of the tokens ids[B, S] given those before them, ``token_logprobs`` of positions 1..S-1:
+        ``(logprobs, entropy, top_logprobs, top_ids)``, [B, S - 1] and [B, S - 1, top].  The mean of ``-logprobs`` is
+        the reference's token NLL (``eval_ppl``, ``benchmarks/eval_llama.py:77-117``).  Overwrites the static cache."""
+        logits = self.prefill(ids, all_logits=True)
+        return token_logprobs(logits[:, :-1], ids[:, 1:], top)
+
+    # ------------------------------------------------------------------ paged cache
+
+    def paged_cache(self, num_pages: int, *, max_seqs: int, page_size: int = 64, max_len: int | None = None,
+                    track_weights: bool = False) -> PagedKVCache:
+        """A paged cache for this rank's kv heads; ``max_len`` slots per sequence (the rotary tables' length unless
+        given).  Positions run to ``max_seq``, whatever is evicted."""
+        return PagedKVCache(len(self.layers), self.nkv_l, self.hd, num_pages=num_pages, max_seqs=max_seqs,
+                            max_len=self.max_seq if max_len is None else max_len, page_size=page_size,
+                            device=self.device, track_weights=track_weights, max_positions=self.max_seq)
+
+    @torch.no_grad()
+    def prefill_paged(self, ids: torch.Tensor, cache: PagedKVCache, seq: int, all_logits: bool = False) -> torch.Tensor:
+        """Run the tokens ids[1, S] as the next ones of sequence ``seq`` (its prompt, or a part of it) and add their
+        keys and values to ``cache``; logits [1, 1 or S, V] of the last (or every) token."""
+        assert ids.dim() == 2 and ids.shape[0] == 1 and ids.shape[1] > 0, ids.shape
+        S, nq, nkv, hd = ids.shape[1], self.nh_l, self.nkv_l, self.hd
+        cache.reserve({seq: S})
+        had = cache.lengths[seq]
+        dev = self.device
+        slots = torch.arange(had, had + S, device=dev, dtype=torch.int32)
+        positions = slots - cache.lens[seq] + cache.positions[seq]
+        seqs = torch.full((S,), seq, device=dev, dtype=torch.int32)
+        n_pages = -(-(had + S) // cache.page_size)
+        mine = cache.table[seq, :n_pages].long()
+        mask = None if had == 0 else torch.arange(had + S, device=dev) <= slots[:, None]
+        h = F.embedding(ids, self.embed)
+        for i, L in enumerate(self.layers):
+            qkv = L["qkv"](rms_norm(h, L["ln1"], self.eps))[0]
+            q = paged_kv_append(qkv, self.cos, self.sin, positions, slots, cache.table, cache.k[i], cache.v[i], seqs=seqs)
+            k, v = (c[i][mine].transpose(0, 1).reshape(nkv, -1, hd)[:, :had + S] for c in (cache.k, cache.v))
+            a = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k[None], v[None], attn_mask=mask,
+                                               is_causal=mask is None, scale=hd ** -0.5, enable_gqa=True)
+            h = h + self._all_reduce(L["o"](a.transpose(1, 2).reshape(1, S, nq * hd)))
+            g, u = L["gu"](rms_norm(h, L["ln2"], self.eps)).chunk(2, dim=-1)
+            h = h + self._all_reduce(L["down"](F.silu(g) * u))
+        cache.lengths[seq] += S
+        cache.seen[seq] += S
+        cache.lens[seq] += S
+        cache.positions[seq] += S
+        cache.live[seq] = 1
+        return self._head(h if all_logits else h[:, -1:])
+
+    @torch.no_grad()
+    def decode_paged(self, ids: torch.Tensor, cache: PagedKVCache, reserve: bool = True) -> torch.Tensor:
+        """One token for every sequence of ``cache``, each at its own position: ids[max_seqs, 1], logits
+        [max_seqs, 1, V].  Rows of sequences that are not live are computed and mean nothing; their cache stays as it
+        is.  ``reserve=False`` leaves the host side to the caller (``cache.reserve_step()``): the rest has no host
+        synchronisation, keeps its addresses and can be captured in a CUDA graph."""
+        assert self.fused, "the paged decode step runs the fused kernels"
+        assert ids.shape == (cache.max_seqs, 1), (tuple(ids.shape), cache.max_seqs)
+        if reserve:
+            cache.reserve_step()
+        live = cache.live > 0
+        slots = torch.where(live, cache.lens, -1)
+        positions = cache.positions.clone()
+        cache.lens.add_(cache.live)
+        cache.positions.add_(cache.live)
+
+        def attend(i: int, qkv: torch.Tensor, att: torch.Tensor) -> None:
+            q = paged_kv_append(qkv, self.cos, self.sin, positions, slots, cache.table, cache.k[i], cache.v[i])
+            paged_decode_attention(q, cache.k[i], cache.v[i], cache.table, cache.lens, out=att.view(q.shape),
+                                   weights=None if cache.weights is None else cache.weights[i])
+
+        x = self._decode_layers_fused(ids, attend)
+        return self._gather_vocab(self.lm_head(x)).view(ids.shape[0], 1, -1)
+
     def _decode_step_fused(self, ids: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         B = ids.shape[0]
         nq, nkv, hd = self.nh_l, self.nkv_l, self.hd
+        q = torch.empty(B, nq, hd, device=self.device, dtype=torch.bfloat16)
+
+        def attend(i: int, qkv: torch.Tensor, att: torch.Tensor) -> None:
+            kc, vc = self.k_cache[i, :B], self.v_cache[i, :B]
+            rope_kv_cache(qkv, self.cos, self.sin, pos, q, kc, vc, nq, nkv)
+            decode_attention(q, kc, vc, pos, att, nq, nkv, hd ** -0.5)
+
+        return self._decode_layers_fused(ids, attend)
+
+    def _decode_layers_fused(self, ids: torch.Tensor, attend) -> torch.Tensor:
+        """Every layer of a single-token step and the final norm; ``attend(layer, qkv, att)`` writes the attention of
+        the layer's projections qkv[B, (nq + 2 nkv) * hd] to att[B, nq * hd] and keeps its keys and values."""
+        B = ids.shape[0]
         cur = F.embedding(ids.view(B), self.embed)  # [B, H], the residual stream (ping-pongs with `other`)
         other = torch.empty_like(cur)
         x = torch.empty_like(cur)
-        q = torch.empty(B, nq, hd, device=cur.device, dtype=torch.bfloat16)
-        att = torch.empty(B, nq * hd, device=cur.device, dtype=torch.bfloat16)
+        att = torch.empty(B, self.nh_l * self.hd, device=cur.device, dtype=torch.bfloat16)
         act = torch.empty(B, self.inter_l, device=cur.device, dtype=torch.bfloat16)
         fold = self.w4 and B <= 32  # norms and SwiGLU run inside the W4 kernels' activation staging
         delta = None
         for i, L in enumerate(self.layers):
-            kc, vc = self.k_cache[i, :B], self.v_cache[i, :B]
             if fold:
                 if delta is None:
                     qkv = w4a16_matmul_prologue(PROLOGUE_RMSNORM, cur, *L["qkv"].q, norm_weight=L["ln1"], eps=self.eps)
@@ -601,8 +692,7 @@ class LlamaTP:
             else:
                 add_rmsnorm(cur, delta, L["ln1"], x, self.eps)
                 qkv = L["qkv"](x)
-            rope_kv_cache(qkv, self.cos, self.sin, pos, q, kc, vc, nq, nkv)
-            decode_attention(q, kc, vc, pos, att, nq, nkv, hd ** -0.5)
+            attend(i, qkv, att)
             fused_ar = fold and self.peers is not None and self.matmul_allreduce
             if fused_ar:
                 o = self._matmul_allreduce_or_none(att, L["o"].q)

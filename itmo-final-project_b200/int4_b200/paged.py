@@ -6,7 +6,8 @@ values lie in fixed-size pages that a block table names:
 * ``paged_kv_append``         rotary embedding of a step's (or a prompt's) tokens, keys and values into their pages;
 * ``paged_decode_attention``  one query token per sequence over its pages, grouped-query, split over the length and
   joined; on request it adds up the attention weight that every cached slot receives;
-* ``paged_evict``             the slots of highest accumulated weight and the most recent ones, copied into new pages.
+* ``paged_evict``             the slots of highest accumulated weight and the most recent ones, copied into new pages;
+* ``PagedKVCache``            the pages of every layer of a model with their bookkeeping, for ``decode.LlamaTP``.
 
 The caches are views ``[pages, kv_heads, page_size, head_dim]`` of any strides that keep a row's ``head_dim`` values
 together (so ``[pages, page_size, kv_heads, head_dim]`` memory transposed will do), bf16 or fp16, head_dim 64 or 128,
@@ -205,3 +206,102 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
                                         _lib.stream_handle(dev))
     _lib.check(st, "paged_evict")
     return new_lens, kept, weights_out
+
+
+class PagedKVCache:
+    """Keys and values of up to ``max_seqs`` sequences, of up to ``max_len`` slots each, in pages of every layer.
+
+    ``k[layer]`` / ``v[layer]`` are ``[num_pages, kv_heads, page_size, head_dim]``; one block table serves all layers.
+    ``lens`` counts a sequence's slots, ``positions`` the tokens that it has seen (its next rotary position); they
+    differ once something was evicted; ``max_positions`` bounds them (the rotary tables' length).  Which pages are free is kept on the host; the tensors that the kernels read
+    (``table``, ``lens``, ``positions``, ``live``) keep their addresses, so a captured step stays valid.  With
+    ``track_weights`` every decode step adds the attention weights up in ``weights[layer]`` ``[max_seqs, kv_heads,
+    slots]`` and ``evict`` can bound the sequences.  ``decode.LlamaTP.paged_cache`` builds one for a model."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, *, num_pages: int, max_seqs: int, max_len: int,
+                 page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device: torch.device | None = None,
+                 track_weights: bool = False, max_positions: int | None = None):
+        _need(dtype in _HALF, "a paged cache holds bfloat16 or float16")
+        _need(head_dim in (64, 128), f"head_dim {head_dim}: 64 and 128 are supported")
+        _need(page_size > 0 and page_size % 8 == 0, f"page size {page_size}: a multiple of 8 is needed")
+        _need(layers > 0 and kv_heads > 0 and num_pages > 0 and 0 < max_seqs <= 4096 and max_len > 0,
+              "layers, kv_heads, num_pages, max_len and max_seqs (at most 4096) must be positive")
+        width = -(-max_len // page_size)
+        _need(not track_weights or width * page_size <= EVICT_MAX_SLOTS,
+              f"max_len {max_len}: eviction selects from at most {EVICT_MAX_SLOTS} slots")
+        dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.page_size, self.max_len, self.max_seqs, self.max_positions = page_size, max_len, max_seqs, max_positions
+        self.k = torch.empty(layers, num_pages, kv_heads, page_size, head_dim, dtype=dtype, device=dev)
+        self.v = torch.empty_like(self.k)
+        self.table = torch.full((max_seqs, width), -1, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(max_seqs, dtype=torch.int32, device=dev)
+        self.positions = torch.zeros(max_seqs, dtype=torch.int32, device=dev)
+        self.live = torch.zeros(max_seqs, dtype=torch.int32, device=dev)  # 1: takes part in decode steps
+        self.weights = torch.zeros(layers, max_seqs, kv_heads, width * page_size, device=dev) if track_weights else None
+        self.free_pages = list(range(num_pages - 1, -1, -1))
+        self.lengths = [0] * max_seqs  # of the host: what `lens` holds
+        self.seen = [0] * max_seqs     # and what `positions` holds
+        self.pages: list[list[int]] = [[] for _ in range(max_seqs)]
+
+    def _missing(self, seq: int, n: int) -> int:
+        _need(0 <= seq < self.max_seqs, f"sequence {seq} of a cache for {self.max_seqs}")
+        if self.lengths[seq] + n > self.max_len:
+            raise _lib.Int4B200Error(f"paged cache: sequence {seq} would hold {self.lengths[seq] + n} slots of {self.max_len}")
+        if self.max_positions is not None and self.seen[seq] + n > self.max_positions:
+            raise _lib.Int4B200Error(f"paged cache: sequence {seq} would reach position {self.seen[seq] + n} of {self.max_positions}")
+        return max(0, -(-(self.lengths[seq] + n) // self.page_size) - len(self.pages[seq]))
+
+    def reserve(self, want: dict[int, int]) -> None:
+        """Pages for ``want[seq]`` more slots of each sequence; all of them, or an error and none."""
+        missing = {seq: self._missing(seq, n) for seq, n in want.items()}
+        if sum(missing.values()) > len(self.free_pages):
+            raise _lib.Int4B200Error(f"paged cache: {sum(missing.values())} pages wanted, {len(self.free_pages)} free")
+        for seq, m in missing.items():
+            if m:
+                at = len(self.pages[seq])
+                self.pages[seq] += [self.free_pages.pop() for _ in range(m)]
+                self.table[seq, at:at + m] = torch.tensor(self.pages[seq][at:], dtype=torch.int32).to(self.table.device)
+
+    def reserve_step(self) -> None:
+        """Host side of a decode step: a slot for every live sequence (before the step, or before its graph replays)."""
+        live = [seq for seq in range(self.max_seqs) if self.pages[seq]]
+        self.reserve({seq: 1 for seq in live})
+        for seq in live:
+            self.lengths[seq] += 1
+            self.seen[seq] += 1
+
+    def free(self, seq: int) -> None:
+        """Forget a sequence; its pages are free again for calls that follow on the same stream."""
+        _need(0 <= seq < self.max_seqs, f"sequence {seq} of a cache for {self.max_seqs}")
+        self.free_pages += reversed(self.pages[seq])
+        self.pages[seq], self.lengths[seq], self.seen[seq] = [], 0, 0
+        self.table[seq] = -1
+        for t in (self.lens, self.positions, self.live):
+            t[seq] = 0
+        if self.weights is not None:
+            self.weights[:, seq].zero_()
+
+    def evict(self, budget: int, recent: int = 0) -> list[int]:
+        """Cut every sequence of more than ``budget`` slots to the ``recent`` last and the ones of highest accumulated
+        weight (``paged_evict``, per layer and kv head); returns the sequences that were cut.  Needs free pages for the
+        kept slots of one sequence at a time; the old pages are free afterwards."""
+        _need(self.weights is not None, "evict needs a cache with track_weights")
+        _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget} and recent {recent}: 0 <= recent <= budget, budget >= 1")
+        cut = [seq for seq in range(self.max_seqs) if self.lengths[seq] > budget]
+        need = -(-budget // self.page_size)
+        for seq in cut:
+            if need > len(self.free_pages):
+                raise _lib.Int4B200Error(f"paged cache: eviction of sequence {seq} wants {need} pages, {len(self.free_pages)} free")
+            fresh = [self.free_pages.pop() for _ in range(need)]
+            new_table = torch.tensor([fresh], dtype=torch.int32).to(self.table.device)
+            row = slice(seq, seq + 1)
+            for layer in range(self.k.shape[0]):
+                w = self.weights[layer, row]
+                paged_evict(w, self.lens[row], self.table[row], self.k[layer], self.v[layer], new_table, budget,
+                            recent=recent, weights_out=w)
+            self.free_pages += reversed(self.pages[seq])
+            self.pages[seq], self.lengths[seq] = fresh, budget
+            self.table[seq, need:] = -1
+            self.table[row, :need] = new_table
+            self.lens[seq] = budget
+        return cut
