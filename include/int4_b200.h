@@ -325,8 +325,8 @@ size_t i4b_paged_attention_workspace_size(int64_t seqs, int64_t nq, int64_t kv_h
                                           int64_t capacity, int with_weights);
 
 /* out[seqs, nq, head_dim] = softmax(q . K^T * scale) . V over slots 0..lens[b]-1 of each sequence, query head h reading
- * kv head h / (nq / kv_heads); zeros where no slot is left.  fp32 softmax; the probabilities are rounded to the cache's
- * type for the product with V.  q: element (b, h, d) at q + b * stride_qb + h * stride_qh + d, strides multiples of 8,
+ * kv head h / (nq / kv_heads), nq / kv_heads <= 1024; zeros where no slot is left.  fp32 softmax; for the product with
+ * V the probabilities are sums of two values of the cache's type.  q: element (b, h, d) at q + b * stride_qb + h * stride_qh + d, strides multiples of 8,
  * 16-byte aligned.  weights, when not NULL: fp32, weights[b * stride_wb + kvh * stride_wh + j] += the probability of
  * slot j summed over the query heads of kv head kvh, j < lens[b]; the rest is left as it was.  Results repeat bit by
  * bit for the same lengths.  workspace: 16-byte aligned. */

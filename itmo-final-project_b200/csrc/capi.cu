@@ -632,7 +632,7 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
                                void* stream) {
   PagedCache c;
   if (int st = paged_cache(cache, &c)) return st;
-  if (nq <= 0 || nq > 65535 || nq % c.kv_heads != 0 || paged_attn_tiles(c, int(nq)) > (1 << 30)) return I4B_ERR_SHAPE;
+  if (nq <= 0 || nq > 65535 || nq % c.kv_heads != 0 || nq / c.kv_heads > 1024 || paged_attn_tiles(c, int(nq)) > (1 << 30)) return I4B_ERR_SHAPE;
   if (c.seqs == 0) return I4B_OK;
   if (!q || !lens || !out || !workspace) return I4B_ERR_INVALID_ARG;
   if (c.seqs == 1) stride_qb = 0;  // never used

@@ -725,38 +725,50 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
   cp_async_wait<0>();
 }
 
-// A group of TPH threads per (sequence, query head): adds the pieces of an item that several runs share, in the runs'
-// order, and writes zeros for an empty sequence.  Most items of a large batch lie in one run and have nothing to add;
-// an item of few long sequences has hundreds of pieces, eight of which each thread has in flight.  TPH = 32 from 2048
-// heads on (8 of them in a CTA), 128 from 512 on, else 512 (one each).
+// Where the pieces of an item lie: none when one run held it whole.
+struct Pieces {
+  int count = 0, first = 0, r0 = 0;
+  __device__ Pieces(const Deal& deal, int t0, int nt) {
+    r0 = deal.run_of(t0);
+    const int r1 = deal.run_of(t0 + nt - 1);
+    if (r0 == r1) return;
+    first = 2 * r0 + (deal.first(r0) == t0 ? 0 : 1);
+    count = r1 - r0 + 1;
+  }
+  __device__ int64_t slot(int i) const { return i == 0 ? first : 2 * (r0 + i); }
+};
+
+struct JoinArgs {
+  int seqs, kv_heads, nq, HT, workers, shared;
+  uint16_t* out;
+  const int* starts;
+  const float* partials;
+};
+
+// A group of TPH threads, thread `tid` of them, for the `at`-th (sequence, query head): adds the pieces of an item that
+// several runs share, in the runs' order, and writes zeros for an empty sequence.  Most items of a large batch lie in
+// one run and have nothing to add; an item of few long sequences has hundreds of pieces, eight of which each thread has
+// in flight.
 template <bool F16, int HD, int TPH>
-__global__ void __launch_bounds__(TPH == 32 ? 256 : TPH)
-    paged_attn_join_kernel(int seqs, int kv_heads, uint16_t* __restrict__ out, int nq, int HT, int workers, int shared,
-                           const int* starts, const float* partials, float* ml) {
-  constexpr int LX = HD / 4;                    // float4 columns
-  constexpr int SL = TPH > LX ? TPH / LX : 1;   // slices over the pieces
-  constexpr int CX = TPH > LX ? 1 : LX / TPH;   // columns per thread
-  static_assert(CX == 1, "a warp covers a head's outputs");
+__device__ __forceinline__ void join_head(const JoinArgs& g, int64_t at, int tid) {
+  constexpr int LX = HD / 4;                   // float4 columns
+  constexpr int SL = TPH > LX ? TPH / LX : 1;  // slices over the pieces
+  static_assert(TPH >= LX, "a warp covers a head's outputs");
   __shared__ float4 acc[TPH > 32 ? SL : 1][LX];
   __shared__ float2 accl[TPH > 32 ? SL : 1];
-  const int64_t at = TPH == 32 ? int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  const int tid = threadIdx.x % TPH;
-  if (at >= int64_t(seqs) * nq) return;
-  const int b = int(at / nq), head = int(at - int64_t(b) * nq);
-  const int G = nq / kv_heads, kvh = head / G, ht = (head % G) / 16, row = (head % G) % 16, prows = min(16, G);
-  pdl_wait();
-  const int start = __ldcg(starts + b), nt = (__ldcg(starts + b + 1) - start) / (kv_heads * HT);
-  const Deal deal(__ldcg(starts + seqs), workers, shared != 0, last_tiles(prows, HD));
-  uint16_t* dst = out + at * HD;
+  const int b = int(at / g.nq), head = int(at - int64_t(b) * g.nq);
+  const int G = g.nq / g.kv_heads, kvh = head / G, ht = (head % G) / 16, row = (head % G) % 16, prows = min(16, G);
+  const int start = __ldcg(g.starts + b), nt = (__ldcg(g.starts + b + 1) - start) / (g.kv_heads * g.HT);
+  uint16_t* dst = g.out + at * HD;
   if (nt == 0) {
     for (int i = tid; i < HD / 2; i += TPH) reinterpret_cast<uint32_t*>(dst)[i] = 0u;
-    if (ml && tid == 0) *reinterpret_cast<float2*>(ml + 2 * at) = make_float2(0.0f, 0.0f);
     return;
   }
-  const int t0 = start + (kvh * HT + ht) * nt, r0 = deal.run_of(t0), r1 = deal.run_of(t0 + nt - 1);
-  if (r0 == r1) return;  // written by the run itself
-  const int first = 2 * r0 + (deal.first(r0) == t0 ? 0 : 1), pieces = r1 - r0 + 1;
-  auto piece = [&](int i) { return partials + int64_t(i == 0 ? first : 2 * (r0 + i)) * piece_floats(prows, HD); };
+  const Deal deal(__ldcg(g.starts + g.seqs), g.workers, g.shared != 0, last_tiles(prows, HD));
+  const Pieces where(deal, start + (kvh * g.HT + ht) * nt, nt);
+  const int pieces = where.count;
+  if (pieces == 0) return;  // written by the run itself
+  auto piece = [&](int i) { return g.partials + where.slot(i) * piece_floats(prows, HD); };
   const int x = tid % LX, s = tid / LX;
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f, mx = -INFINITY;  // this thread's pieces, relative to their largest max
@@ -778,8 +790,8 @@ __global__ void __launch_bounds__(TPH == 32 ? 256 : TPH)
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) top = fmaxf(top, e[k].x);
-    const float base = top == -INFINITY ? 0.0f : top, g = ex2(mx - base);
-    a.x *= g, a.y *= g, a.z *= g, a.w *= g, l *= g;
+    const float base = top == -INFINITY ? 0.0f : top, k0 = ex2(mx - base);
+    a.x *= k0, a.y *= k0, a.z *= k0, a.w *= k0, l *= k0;
     mx = top;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
@@ -812,35 +824,109 @@ __global__ void __launch_bounds__(TPH == 32 ? 256 : TPH)
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   *reinterpret_cast<uint2*>(dst + 4 * x) = make_uint2(pack2<F16>(a.x * inv, a.y * inv), pack2<F16>(a.z * inv, a.w * inv));
-  if (ml && x == 0) *reinterpret_cast<float2*>(ml + 2 * at) = make_float2(mx, inv);
 }
 
-// weights[b, kvh, j] += sum over the kv head's query heads of exp2(s_j - m) / l, from the stored scaled scores.
-__global__ void __launch_bounds__(256) paged_attn_weights_kernel(const PagedCache c, const int32_t* __restrict__ lens,
-                                                                 int nq, const float* __restrict__ logits,
-                                                                 int64_t logit_stride, const float* __restrict__ ml,
-                                                                 float* __restrict__ weights, int64_t swb, int64_t swh) {
-  const int b = blockIdx.z, kvh = blockIdx.y, G = nq / c.kv_heads;
+// TPH = 32 from 2048 heads on (8 of them in a CTA), 128 from 512 on, else 512 (one each).
+template <bool F16, int HD, int TPH>
+__global__ void __launch_bounds__(TPH == 32 ? 256 : TPH) paged_attn_join_kernel(const JoinArgs g) {
+  const int64_t at = TPH == 32 ? int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (at >= int64_t(g.seqs) * g.nq) return;
   pdl_wait();
-  const int L = clamped_len(c, lens, b), j = 4 * (blockIdx.x * 256 + threadIdx.x);
-  if (j >= L) return;
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int r = 0; r < G; ++r) {
-    const int64_t row = int64_t(b) * nq + kvh * G + r;
-    const float2 e = __ldcg(reinterpret_cast<const float2*>(ml + 2 * row));
-    const float4 s = __ldcg(reinterpret_cast<const float4*>(logits + row * logit_stride + j));
-    const float base = e.x == -INFINITY ? 0.0f : e.x;
-    sum.x = fmaf(ex2(s.x - base), e.y, sum.x);
-    sum.y = fmaf(ex2(s.y - base), e.y, sum.y);
-    sum.z = fmaf(ex2(s.z - base), e.y, sum.z);
-    sum.w = fmaf(ex2(s.w - base), e.y, sum.w);
+  join_head<F16, HD, TPH>(g, at, threadIdx.x % TPH);
+}
+
+// weights[b, kvh, j] += sum over the kv head's query heads of exp2(s_j - m) / l, from the stored scaled scores, for the
+// positions 4 (thread + 256 x), x = part, part + parts, ...; ml[r] = (m, 1 / l) of the kv head's r-th query head.
+__device__ __forceinline__ void add_weights(const float2* ml, int G, const float* scores, int64_t score_stride, int L,
+                                            float* w, int part, int parts) {
+  for (int j = 4 * (part * 256 + int(threadIdx.x)); j < L; j += 1024 * parts) {
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int r = 0; r < G; ++r) {
+      const float2 e = ml[r];
+      const float4 s = __ldcg(reinterpret_cast<const float4*>(scores + r * score_stride + j));
+      const float base = e.x == -INFINITY ? 0.0f : e.x;
+      sum.x = fmaf(ex2(s.x - base), e.y, sum.x);
+      sum.y = fmaf(ex2(s.y - base), e.y, sum.y);
+      sum.z = fmaf(ex2(s.z - base), e.y, sum.z);
+      sum.w = fmaf(ex2(s.w - base), e.y, sum.w);
+    }
+    const int n = min(4, L - j);
+    w[j] += sum.x;
+    if (n > 1) w[j + 1] += sum.y;
+    if (n > 2) w[j + 2] += sum.z;
+    if (n > 3) w[j + 3] += sum.w;
   }
-  float* w = weights + b * swb + kvh * swh + j;
-  const int n = min(4, L - j);
-  w[0] += sum.x;
-  if (n > 1) w[1] += sum.y;
-  if (n > 2) w[2] += sum.z;
-  if (n > 3) w[3] += sum.w;
+}
+
+constexpr int kMaxGroup = 1024;  // query heads per kv head
+
+struct WeightArgs {
+  const float* logits;
+  int64_t logit_stride;
+  const float2* ml;
+  float* weights;
+  int64_t swb, swh;
+  int parts;  // CTAs per (sequence, kv head)
+};
+
+// After whole items alone: (m, 1 / l) of every head is there.
+__global__ void __launch_bounds__(256) paged_attn_weights_kernel(const PagedCache c, const int32_t* __restrict__ lens,
+                                                                 int nq, const WeightArgs a) {
+  const int item = int(blockIdx.x), b = item / c.kv_heads, kvh = item % c.kv_heads, G = nq / c.kv_heads;
+  __shared__ float2 ml[kMaxGroup];
+  pdl_wait();
+  for (int r = threadIdx.x; r < G; r += 256) ml[r] = __ldcg(a.ml + int64_t(b) * nq + kvh * G + r);
+  __syncthreads();
+  add_weights(ml, G, a.logits + (int64_t(b) * nq + kvh * G) * a.logit_stride, a.logit_stride, clamped_len(c, lens, b),
+              a.weights + b * a.swb + kvh * a.swh, 0, 1);
+}
+
+// The join and the weights in one launch: the first CTAs join (TPH = 32 from 512 heads on, else 256), the others add
+// the weights of a (sequence, kv head) each, for which they add up the pieces' sums (not the outputs) themselves.
+template <bool F16, int HD, int TPH>
+__global__ void __launch_bounds__(256) paged_attn_finish_kernel(const PagedCache c, const int32_t* __restrict__ lens,
+                                                                const JoinArgs g, int join_ctas, const WeightArgs a) {
+  __shared__ float2 ml[kMaxGroup];
+  pdl_wait();
+  if (int(blockIdx.x) < join_ctas) {
+    const int64_t at = TPH == 32 ? int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+    if (at < int64_t(g.seqs) * g.nq) join_head<F16, HD, TPH>(g, at, threadIdx.x % TPH);
+    return;
+  }
+  const int id = int(blockIdx.x) - join_ctas, item = id / a.parts, b = item / g.kv_heads, kvh = item % g.kv_heads;
+  const int G = g.nq / g.kv_heads, prows = min(16, G), lane = threadIdx.x & 31;
+  const int L = clamped_len(c, lens, b);
+  if (4 * 256 * (id % a.parts) >= L) return;
+  const int start = __ldcg(g.starts + b), nt = (__ldcg(g.starts + b + 1) - start) / (g.kv_heads * g.HT);
+  const Deal deal(__ldcg(g.starts + g.seqs), g.workers, g.shared != 0, last_tiles(prows, HD));
+  for (int r = threadIdx.x >> 5; r < G; r += 8) {  // a warp per head
+    const Pieces where(deal, start + (kvh * g.HT + r / 16) * nt, nt);
+    if (where.count == 0) {
+      if (lane == 0) ml[r] = __ldcg(a.ml + int64_t(b) * g.nq + kvh * G + r);
+      continue;
+    }
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll 4
+    for (int i = lane; i < where.count; i += 32) {
+      const float2 e = __ldcg(reinterpret_cast<const float2*>(g.partials + where.slot(i) * piece_floats(prows, HD) + prows * HD +
+                                                              2 * (r % 16)));
+      const float top = fmaxf(m, e.x), base = top == -INFINITY ? 0.0f : top;
+      l = l * ex2(m - base) + e.y * ex2(e.x - base);
+      m = top;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, o), l2 = __shfl_xor_sync(0xFFFFFFFFu, l, o);
+      const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
+      l = l * ex2(m - base) + l2 * ex2(m2 - base);
+      m = top;
+    }
+    if (lane == 0) ml[r] = make_float2(m, l > 0.0f || l != l ? 1.0f / l : 0.0f);
+  }
+  __syncthreads();
+  add_weights(ml, G, a.logits + (int64_t(b) * g.nq + kvh * G) * a.logit_stride, a.logit_stride, L,
+              a.weights + b * a.swb + kvh * a.swh, id % a.parts, a.parts);
 }
 
 // ------------------------------------------------------------------ eviction
@@ -1147,18 +1233,24 @@ cudaError_t attn(const PagedCache& c, const PagedAttn& a, const PagedAttnWorkspa
   kern<<<ctas, kAttnWarps * 32, smem, s>>>(c, a.q, a.sqb, a.sqh, a.lens, a.out, a.nq, HT, a.scale * 1.4426950408889634f,
                                            w.partials, w.logits, w.logit_stride, w.ml, w.counter, w.starts);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if (!whole) {
-    const int64_t heads = int64_t(c.seqs) * a.nq;
-    auto join = heads >= 2048 ? paged_attn_join_kernel<F16, HD, 32>
-                              : (heads >= 512 ? paged_attn_join_kernel<F16, HD, 128> : paged_attn_join_kernel<F16, HD, 512>);
-    e = launch_after(join, dim3(unsigned(heads >= 2048 ? (heads + 7) / 8 : heads)), dim3(heads >= 2048 ? 256 : (heads >= 512 ? 128 : 512)),
-                     0, s, c.seqs, c.kv_heads, a.out, a.nq, HT, workers, w.counter ? 1 : 0,
-                     static_cast<const int*>(w.starts), static_cast<const float*>(w.partials), w.ml);
+  const int64_t heads = int64_t(c.seqs) * a.nq;
+  const JoinArgs g = {c.seqs, c.kv_heads, a.nq, HT, workers, w.counter ? 1 : 0, a.out, w.starts, w.partials};
+  const int items = c.seqs * c.kv_heads;
+  WeightArgs wa = {w.logits, w.logit_stride, reinterpret_cast<const float2*>(w.ml), a.weights, a.swb, a.swh, 1};
+  if (WEIGHTS) {
+    if (c.capacity == 0) return cudaSuccess;
+    if (whole) return launch_after(paged_attn_weights_kernel, dim3(unsigned(items)), dim3(256), 0, s, c, a.lens, a.nq, wa);
+    // four CTAs per SM over all items, whatever the tables could hold
+    wa.parts = std::max(1, std::min((c.capacity + 1023) / 1024, 4 * sms / items));
+    const int joins = int(heads >= 512 ? (heads + 7) / 8 : heads);
+    return launch_after(heads >= 512 ? paged_attn_finish_kernel<F16, HD, 32> : paged_attn_finish_kernel<F16, HD, 256>,
+                        dim3(unsigned(joins + items * wa.parts)), dim3(256), 0, s, c, a.lens, g, joins, wa);
   }
-  if (e != cudaSuccess || !WEIGHTS || c.capacity == 0) return e;
-  return launch_after(paged_attn_weights_kernel, dim3(unsigned((c.capacity + 1023) / 1024), unsigned(c.kv_heads), unsigned(c.seqs)),
-                      dim3(256), 0, s, c, a.lens, a.nq, static_cast<const float*>(w.logits), w.logit_stride,
-                      static_cast<const float*>(w.ml), a.weights, a.swb, a.swh);
+  if (whole) return cudaSuccess;
+  if (heads >= 2048)
+    return launch_after(paged_attn_join_kernel<F16, HD, 32>, dim3(unsigned((heads + 7) / 8)), dim3(256), 0, s, g);
+  if (heads >= 512) return launch_after(paged_attn_join_kernel<F16, HD, 128>, dim3(unsigned(heads)), dim3(128), 0, s, g);
+  return launch_after(paged_attn_join_kernel<F16, HD, 512>, dim3(unsigned(heads)), dim3(512), 0, s, g);
 }
 
 template <bool F16, int HD>
