@@ -319,8 +319,9 @@ int i4b_paged_kv_append(const i4b_paged_cache* cache, const void* qkv, int64_t s
                         const void* cos_table, const void* sin_table, int table_dtype, int64_t max_pos,
                         const int32_t* positions, const int32_t* slots, const int32_t* seqs, void* q_out, void* stream);
 
-/* Bytes of workspace i4b_paged_decode_attention needs (0: sizes not supported, or no B200).  Needs no clearing; calls
- * that share a workspace must not overlap in time. */
+/* Bytes of workspace i4b_paged_decode_attention needs: 0 for tables of up to 256 slots (128 at head_dim 128) without
+ * weights (and for sizes that are not supported, or without a B200).  Needs no clearing; calls that share a workspace
+ * must not overlap in time. */
 size_t i4b_paged_attention_workspace_size(int64_t seqs, int64_t nq, int64_t kv_heads, int64_t head_dim,
                                           int64_t capacity, int with_weights);
 

@@ -634,7 +634,7 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
   if (int st = paged_cache(cache, &c)) return st;
   if (nq <= 0 || nq > 65535 || nq % c.kv_heads != 0 || nq / c.kv_heads > 1024 || paged_attn_tiles(c, int(nq)) > (1 << 30)) return I4B_ERR_SHAPE;
   if (c.seqs == 0) return I4B_OK;
-  if (!q || !lens || !out || !workspace) return I4B_ERR_INVALID_ARG;
+  if (!q || !lens || !out) return I4B_ERR_INVALID_ARG;
   if (c.seqs == 1) stride_qb = 0;  // never used
   if (nq == 1) stride_qh = 0;
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || stride_qb < 0 || stride_qh < 0 || stride_qb % 8 != 0 || stride_qh % 8 != 0)
@@ -642,9 +642,10 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
   DevInfo d;
   if (int st = current_device_info(&d)) return st;
   PagedAttnWorkspace w;
-  if (workspace_bytes < paged_attn_workspace(c.seqs, int(nq), c.kv_heads, c.head_dim, c.capacity, weights != nullptr, d.sms,
-                                             workspace, &w))
-    return I4B_ERR_WORKSPACE;
+  const size_t need = paged_attn_workspace(c.seqs, int(nq), c.kv_heads, c.head_dim, c.capacity, weights != nullptr, d.sms,
+                                           workspace, &w);
+  if (need > 0 && !workspace) return I4B_ERR_INVALID_ARG;
+  if (workspace_bytes < need) return I4B_ERR_WORKSPACE;
   const PagedAttn a = {static_cast<const uint16_t*>(q), stride_qb, stride_qh, lens, static_cast<uint16_t*>(out), int(nq),
                        scale, weights, stride_wb, stride_wh};
   const cudaError_t e = launch_paged_attn(c, a, w, d.sms, static_cast<cudaStream_t>(stream));

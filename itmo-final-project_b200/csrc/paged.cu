@@ -1275,11 +1275,12 @@ size_t paged_attn_workspace(int seqs, int nq, int kv_heads, int head_dim, int ca
   const int G = nq / kv_heads, tile = tile_of(head_dim), HT = (G + 15) / 16;
   const int64_t workers = int64_t(sms) * kAttnCtas * kAttnWarps;
   const int64_t stride = (int64_t(capacity) + tile - 1) / tile * tile;
+  const bool whole = capacity <= kWholeTiles * tile;
   // the lengths are on the device: runs are shared where the tables' whole capacity would call for it
   const int last = last_tiles(std::min(G, 16), head_dim);
-  const bool shared = capacity > kWholeTiles * tile && int64_t(seqs) * (stride / tile) * kv_heads * HT >= workers * 8 * last;
-  const int64_t pieces = 2 * workers * (shared ? kMostRuns : 1);
-  const size_t b0 = up256(size_t(pieces) * piece_floats(std::min(G, 16), head_dim) * 4), b1 = 256 + up256(4 * (size_t(seqs) + 1));
+  const bool shared = !whole && int64_t(seqs) * (stride / tile) * kv_heads * HT >= workers * 8 * last;
+  const int64_t pieces = whole ? 0 : 2 * workers * (shared ? kMostRuns : 1);
+  const size_t b0 = up256(size_t(pieces) * piece_floats(std::min(G, 16), head_dim) * 4), b1 = whole ? 0 : 256 + up256(4 * (size_t(seqs) + 1));
   const size_t b2 = weights ? up256(size_t(seqs) * nq * size_t(stride) * 4) : 0;
   const size_t b3 = weights ? up256(size_t(seqs) * nq * 8) : 0;
   if (w) {

@@ -142,9 +142,12 @@ def stream_handle(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """Context in which ``device`` is the current one (nothing to do, and nothing spent, where it is already)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 # Per (device, stream) workspace, zero-filled once; the kernels leave their

@@ -59,14 +59,19 @@ def _table(t: torch.Tensor, name: str) -> None:
 
 
 def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> bytes:
-    _need(k.dim() == 4 and k.shape == v.shape, "k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim]")
-    _need(k.dtype in _HALF and v.dtype == k.dtype, "k_cache and v_cache must both be bfloat16 or both float16")
+    if not (k.dim() == 4 and k.shape == v.shape):
+        raise ValueError("k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim]")
+    if not (k.dtype in _HALF and v.dtype == k.dtype):
+        raise ValueError("k_cache and v_cache must both be bfloat16 or both float16")
     _table(table, "block_table")
     pages, heads, page, dim = k.shape
-    _need(dim in (64, 128), f"head_dim {dim}: 64 and 128 are supported")
-    _need(page > 0 and page % 8 == 0, f"page size {page}: a multiple of 8 is needed")
+    if not (dim in (64, 128)):
+        raise ValueError(f"head_dim {dim}: 64 and 128 are supported")
+    if not (page > 0 and page % 8 == 0):
+        raise ValueError(f"page size {page}: a multiple of 8 is needed")
     ks, vs = k.stride(), v.stride()
-    _need(ks[3] == 1 and vs[3] == 1, "the caches' last dimension must have unit stride")
+    if not (ks[3] == 1 and vs[3] == 1):
+        raise ValueError("the caches' last dimension must have unit stride")
     seqs, width = table.shape
     return _lib.PAGED_CACHE.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.data_ptr(),
                                  table.stride(0), pages, heads, page, dim, seqs, width, _lib.DTYPE_CODE[k.dtype])
@@ -92,24 +97,28 @@ def paged_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos
     tables gives a zero query and writes nothing.  Two tokens of a call must not name the same slot of a sequence."""
     c = _cache(k_cache, v_cache, block_table)
     nkv, dim = k_cache.shape[1], k_cache.shape[3]
-    _need(qkv.dim() == 2 and qkv.dtype == k_cache.dtype, "qkv must be [tokens, (nq + 2 nkv) * head_dim] of the caches' dtype")
+    if not (qkv.dim() == 2 and qkv.dtype == k_cache.dtype):
+        raise ValueError("qkv must be [tokens, (nq + 2 nkv) * head_dim] of the caches' dtype")
     T, width = qkv.shape
     nq = width // dim - 2 * nkv
-    _need(width % dim == 0 and nq > 0, f"qkv rows of {width} values do not hold {nkv} key and value heads of {dim} and queries")
-    _need(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == dim and cos.shape[0] > 0
-          and cos.dtype == sin.dtype and cos.dtype in (k_cache.dtype, torch.float32) and cos.is_contiguous()
-          and sin.is_contiguous(), "cos and sin must be contiguous [max_pos, head_dim], of the caches' dtype or float32")
+    if not (width % dim == 0 and nq > 0):
+        raise ValueError(f"qkv rows of {width} values do not hold {nkv} key and value heads of {dim} and queries")
+    if not (cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == dim and cos.shape[0] > 0
+            and cos.dtype == sin.dtype and cos.dtype in (k_cache.dtype, torch.float32) and cos.is_contiguous()
+            and sin.is_contiguous()):
+        raise ValueError("cos and sin must be contiguous [max_pos, head_dim], of the caches' dtype or float32")
     _indices(positions, "positions", T)
     _indices(slots, "slots", T)
     if seqs is not None:
         _indices(seqs, "seqs", T)
     else:
-        _need(T <= block_table.shape[0], f"{T} tokens without seqs, and a block table of {block_table.shape[0]} sequences")
+        if not (T <= block_table.shape[0]):
+            raise ValueError(f"{T} tokens without seqs, and a block table of {block_table.shape[0]} sequences")
     if out is None:
         out = qkv.new_empty((T, nq, dim))
     else:
-        _need(out.shape == (T, nq, dim) and out.dtype == qkv.dtype and out.is_contiguous(),
-              "out must be a contiguous [tokens, nq, head_dim] of the caches' dtype")
+        if not (out.shape == (T, nq, dim) and out.dtype == qkv.dtype and out.is_contiguous()):
+            raise ValueError("out must be a contiguous [tokens, nq, head_dim] of the caches' dtype")
     dev = qkv.device
     _on_gpu(dev, k_cache, v_cache, block_table, cos, sin, positions, slots, seqs, out)
     qkv = _rows16(qkv)
@@ -135,32 +144,33 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     c = _cache(k_cache, v_cache, block_table)
     nkv, page, dim = k_cache.shape[1:]
     B, width = block_table.shape
-    _need(q.dim() == 3 and q.shape[0] == B and q.shape[2] == dim and q.dtype == k_cache.dtype,
-          "q must be [sequences, nq, head_dim] of the caches' dtype")
+    if not (q.dim() == 3 and q.shape[0] == B and q.shape[2] == dim and q.dtype == k_cache.dtype):
+        raise ValueError("q must be [sequences, nq, head_dim] of the caches' dtype")
     nq = q.shape[1]
-    _need(nq > 0 and nq % nkv == 0, f"{nq} query heads do not divide over {nkv} kv heads")
+    if not (nq > 0 and nq % nkv == 0):
+        raise ValueError(f"{nq} query heads do not divide over {nkv} kv heads")
     _indices(lens, "lens", B)
     if weights is not None:
-        _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
-              and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1),
-              f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
+        if not (weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
+                and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1)):
+            raise ValueError(f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _need(out.shape == (B, nq, dim) and out.dtype == q.dtype and out.is_contiguous(),
-              "out must be a contiguous [sequences, nq, head_dim] of the caches' dtype")
+        if not (out.shape == (B, nq, dim) and out.dtype == q.dtype and out.is_contiguous()):
+            raise ValueError("out must be a contiguous [sequences, nq, head_dim] of the caches' dtype")
     dev = q.device
     _on_gpu(dev, k_cache, v_cache, block_table, lens, weights, out)
     q = _rows16(q)
     need = _attention_workspace(B, nq, nkv, dim, width * page, weights is not None, dev.index)
     # from torch's allocator each time: two captured graphs never share it, and eager streams do not either
-    ws = lens.new_empty(need, dtype=torch.uint8)
+    ws = lens.new_empty(need, dtype=torch.uint8) if need else None
     with _lib.on_device(dev):
         st = _lib.lib().i4b_paged_decode_attention(c, q.data_ptr(), q.stride(0), q.stride(1), nq, lens.data_ptr(),
                                           dim ** -0.5 if scale is None else scale, out.data_ptr(),
                                           None if weights is None else weights.data_ptr(),
                                           0 if weights is None else weights.stride(0),
-                                          0 if weights is None else weights.stride(1), ws.data_ptr(), need,
+                                          0 if weights is None else weights.stride(1), None if ws is None else ws.data_ptr(), need,
                                           _lib.stream_handle(dev))
     _lib.check(st, "paged_decode_attention")
     return out
@@ -180,21 +190,24 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
     c = _cache(k_cache, v_cache, block_table)
     nkv, page = k_cache.shape[1:3]
     B, width = block_table.shape
-    _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
-          and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1),
-          f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
-    _need(width * page <= EVICT_MAX_SLOTS, f"{width * page} slots per sequence: eviction selects from at most {EVICT_MAX_SLOTS}")
+    if not (weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
+            and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1)):
+        raise ValueError(f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
+    if not (width * page <= EVICT_MAX_SLOTS):
+        raise ValueError(f"{width * page} slots per sequence: eviction selects from at most {EVICT_MAX_SLOTS}")
     _indices(lens, "lens", B)
     _table(new_table, "new_table")
-    _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget} and recent {recent}: 0 <= recent <= budget, budget >= 1")
-    _need(new_table.shape[0] == B and new_table.shape[1] * page >= budget,
-          f"new_table must hold {-(-budget // page)} pages for each of {B} sequences")
+    if not (budget >= 1 and 0 <= recent <= budget):
+        raise ValueError(f"budget {budget} and recent {recent}: 0 <= recent <= budget, budget >= 1")
+    if not (new_table.shape[0] == B and new_table.shape[1] * page >= budget):
+        raise ValueError(f"new_table must hold {-(-budget // page)} pages for each of {B} sequences")
     dev = weights.device
     if weights_out is None:
         weights_out = torch.empty_like(weights, memory_format=torch.contiguous_format)
     else:
-        _need(weights_out.shape == weights.shape and weights_out.dtype == torch.float32
-              and (weights.shape[2] <= 1 or weights_out.stride(2) == 1), "weights_out must be float32 of the weights' shape")
+        if not (weights_out.shape == weights.shape and weights_out.dtype == torch.float32
+                and (weights.shape[2] <= 1 or weights_out.stride(2) == 1)):
+            raise ValueError("weights_out must be float32 of the weights' shape")
     _on_gpu(dev, k_cache, v_cache, block_table, lens, new_table, weights_out)
     new_lens = torch.empty_like(lens)
     kept = lens.new_empty((B, nkv, budget))
