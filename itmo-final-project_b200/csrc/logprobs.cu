@@ -20,7 +20,7 @@ namespace i4b {
 namespace {
 
 constexpr int kCand = 512;  // candidates above, and at, the threshold that a CTA holds
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float ex2(float v) {
   float r;
@@ -42,11 +42,6 @@ __device__ __forceinline__ float2 unpack(uint64_t v) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
@@ -136,15 +131,18 @@ __device__ __forceinline__ Stat merge(const Stat& x, const Stat& y) {
   return r;
 }
 
-// N chunks at once: their maximum first, then 4.5 instructions per element.  A -inf, a NaN or a +inf among them makes
-// the sums of a NaN; such a batch is taken again one by one.
+// N chunks at once: their maximum first, then, in units of log 2, t = z log2(e) - m log2(e) in one packed operation of
+// two elements, as are the two sums: 3.75 instructions per element.  m log2(e) is rounded, off by delta, and with it
+// every t: the sums are put right for that afterwards.  A -inf, a NaN or a +inf among the logits, or one so large that t
+// overflows, leaves no finite sum; such a batch is taken again one by one.
 template <typename E, int N>
 __device__ __forceinline__ void add_batch(Stat& st, const uint4 (&w)[N]) {
   float top = E::most(w[0]);
 #pragma unroll
   for (int u = 1; u < N; ++u) top = fmaxf(top, E::most(w[u]));
   if (top > st.m) raise(st, top);
-  const uint64_t nm = pack(-st.m, -st.m), l2 = pack(kLog2e, kLog2e);
+  const float ml = st.m * kLog2e, delta = fmaf(st.m, kLog2e, -ml);
+  const uint64_t nm = pack(-ml, -ml), l2 = pack(kLog2e, kLog2e);
   uint64_t s2 = 0, a2 = 0;
 #pragma unroll
   for (int u = 0; u < N; ++u) {
@@ -152,18 +150,19 @@ __device__ __forceinline__ void add_batch(Stat& st, const uint4 (&w)[N]) {
     E::many(w[u], f);
 #pragma unroll
     for (int i = 0; i < E::kVec; i += 2) {
-      const uint64_t d = add2(pack(f[i], f[i + 1]), nm);
-      const float2 t = unpack(mul2(d, l2));
+      const uint64_t t2 = fma2(pack(f[i], f[i + 1]), l2, nm);
+      const float2 t = unpack(t2);
       const uint64_t e = pack(ex2(t.x), ex2(t.y));
       s2 = add2(s2, e);
-      a2 = fma2(e, d, a2);
+      a2 = fma2(e, t2, a2);
     }
   }
   const float2 s = unpack(s2), a = unpack(a2);
-  const float as = a.x + a.y;
-  if (as == as) {
-    st.s += s.x + s.y;
-    st.a += as;
+  const float ss = s.x + s.y, as = a.x + a.y;
+  if (as - as == 0.0f) {  // finite
+    const float back = 1.0f - delta * kLn2;  // 2^-delta
+    st.s = fmaf(ss, back, st.s);
+    st.a = fmaf((as - delta * ss) * kLn2, back, st.a);
   } else {
 #pragma unroll 1
     for (int u = 0; u < N; ++u) {
