@@ -73,85 +73,95 @@ __device__ __forceinline__ int page_entry(const PagedCache& c, const int32_t* ro
 
 // ------------------------------------------------------------------ append
 
-// One CTA per token; a thread owns 8 dims of the head's first half and the matching 8 of the second (two 16-byte
-// loads), so that rotate_half needs no exchange.  Rotation in fp32, rounded once.  Bound by bytes: every value is
-// read once and written once; the token's row of the two tables comes from L1 after the first head.
+// A thread owns 8 dims of a head's first half and the matching 8 of the second (two 16-byte loads), so that
+// rotate_half needs no exchange, for kHeads heads of one token, whose angles it reads once.  Rotation in fp32, rounded
+// once.  Bound by bytes: every value is read once and written once, and a thread has all of its own in flight.
+// 16381 tokens of 32 + 2 x 8 heads of 64 (206 MB; a plain copy of as much takes 34.9 us), heads per thread x threads:
+// 6 x 128 34.8 us, 7 x 128 34.8, 6 x 256 36.1, 5 x 256 38.0, 4 x 256 41.1, 2 x 128 41.1, 8 x 128 43.9, 1 x 192 41.5.
+constexpr int kAppendThreads = 128;
+constexpr int kHeads = 6;
+
 template <bool F16, bool T32, int HD>
-__global__ void __launch_bounds__(256) paged_append_kernel(const PagedCache c, const uint16_t* __restrict__ qkv,
-                                                           int64_t sqkv, const void* __restrict__ cosT,
-                                                           const void* __restrict__ sinT, int max_pos,
-                                                           const int32_t* __restrict__ positions,
-                                                           const int32_t* __restrict__ slots,
-                                                           const int32_t* __restrict__ seqs,
-                                                           uint16_t* __restrict__ q_out, int nq) {
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(
+    const PagedCache c, const uint16_t* __restrict__ qkv, int64_t sqkv, int64_t tokens, const void* __restrict__ cosT,
+    const void* __restrict__ sinT, int max_pos, const int32_t* __restrict__ positions, const int32_t* __restrict__ slots,
+    const int32_t* __restrict__ seqs, uint16_t* __restrict__ q_out, int nq, int per_token) {
   constexpr int TPH = HD / 16;  // threads per head
-  const int64_t tok = blockIdx.x;
-  const int p = positions[tok], slot = slots[tok], seq = seqs ? seqs[tok] : int(tok);
+  const int64_t at = int64_t(blockIdx.x) * kAppendThreads + threadIdx.x, tok = at / per_token;
+  if (tok >= tokens) return;
+  const int unit = int(at - tok * per_token), ch = unit % TPH, h0 = unit / TPH, step = per_token / TPH;
+  const int heads = nq + 2 * c.kv_heads;
+  const int p = __ldg(positions + tok), slot = __ldg(slots + tok), seq = seqs ? __ldg(seqs + tok) : int(tok);
+  const uint16_t* src0 = qkv + tok * sqkv + 8 * ch;
+  uint4 x0[kHeads], x1[kHeads];
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    const int h = h0 + k * step;
+    if (h < heads) {
+      x0[k] = __ldg(reinterpret_cast<const uint4*>(src0 + int64_t(h) * HD));
+      x1[k] = __ldg(reinterpret_cast<const uint4*>(src0 + int64_t(h) * HD + HD / 2));
+    }
+  }
   const bool rot_ok = uint32_t(p) < uint32_t(max_pos);
+  float co0[8], co1[8], si0[8], si1[8];
+  if (rot_ok) {
+    if constexpr (T32) {
+      const float* cp = static_cast<const float*>(cosT) + int64_t(p) * HD + 8 * ch;
+      const float* sp = static_cast<const float*>(sinT) + int64_t(p) * HD + 8 * ch;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        *reinterpret_cast<float4*>(co0 + e) = __ldg(reinterpret_cast<const float4*>(cp + e));
+        *reinterpret_cast<float4*>(co1 + e) = __ldg(reinterpret_cast<const float4*>(cp + HD / 2 + e));
+        *reinterpret_cast<float4*>(si0 + e) = __ldg(reinterpret_cast<const float4*>(sp + e));
+        *reinterpret_cast<float4*>(si1 + e) = __ldg(reinterpret_cast<const float4*>(sp + HD / 2 + e));
+      }
+    } else {
+      const uint16_t* cp = static_cast<const uint16_t*>(cosT) + int64_t(p) * HD + 8 * ch;
+      const uint16_t* sp = static_cast<const uint16_t*>(sinT) + int64_t(p) * HD + 8 * ch;
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(cp)), b = __ldg(reinterpret_cast<const uint4*>(cp + HD / 2));
+      const uint4 d = __ldg(reinterpret_cast<const uint4*>(sp)), f = __ldg(reinterpret_cast<const uint4*>(sp + HD / 2));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        *reinterpret_cast<float2*>(co0 + 2 * w) = unpack2<F16>(reinterpret_cast<const uint32_t*>(&a)[w]);
+        *reinterpret_cast<float2*>(co1 + 2 * w) = unpack2<F16>(reinterpret_cast<const uint32_t*>(&b)[w]);
+        *reinterpret_cast<float2*>(si0 + 2 * w) = unpack2<F16>(reinterpret_cast<const uint32_t*>(&d)[w]);
+        *reinterpret_cast<float2*>(si1 + 2 * w) = unpack2<F16>(reinterpret_cast<const uint32_t*>(&f)[w]);
+      }
+    }
+  }
   int page = -1, row = 0;
-  if (uint32_t(seq) < uint32_t(c.seqs) && uint32_t(slot) < uint32_t(c.capacity)) {
+  if (rot_ok && uint32_t(seq) < uint32_t(c.seqs) && uint32_t(slot) < uint32_t(c.capacity)) {
     const int pi = page_of(c, slot);
     page = page_entry(c, c.table + int64_t(seq) * c.table_stride, pi);
     row = slot - pi * c.page_size;
   }
-  if (!rot_ok) page = -1;
-  const int heads = nq + 2 * c.kv_heads;
-  const uint16_t* src0 = qkv + tok * sqkv;
-  for (int i = threadIdx.x; i < heads * TPH; i += blockDim.x) {
-    const int h = i / TPH, ch = i % TPH;
-    const uint16_t* src = src0 + int64_t(h) * HD + 8 * ch;
-    uint4 x0 = __ldg(reinterpret_cast<const uint4*>(src));
-    uint4 x1 = __ldg(reinterpret_cast<const uint4*>(src + HD / 2));
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    const int h = h0 + k * step;
+    if (h >= heads) break;
     uint16_t* dst;
-    if (h >= nq + c.kv_heads) {
-      if (page < 0) continue;
+    if (h < nq)
+      dst = q_out + (tok * nq + h) * HD + 8 * ch;
+    else if (page < 0)
+      continue;
+    else if (h < nq + c.kv_heads)
+      dst = c.k + page * c.ks_page + int64_t(h - nq) * c.ks_head + int64_t(row) * c.ks_token + 8 * ch;
+    else
       dst = c.v + page * c.vs_page + int64_t(h - nq - c.kv_heads) * c.vs_head + int64_t(row) * c.vs_token + 8 * ch;
-    } else {
-      if (h >= nq) {
-        if (page < 0) continue;
-        dst = c.k + page * c.ks_page + int64_t(h - nq) * c.ks_head + int64_t(row) * c.ks_token + 8 * ch;
-      } else {
-        dst = q_out + (tok * nq + h) * HD + 8 * ch;
-      }
-      if (!rot_ok) {  // a position without an angle: the query is zero, nothing is cached
-        x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
-      } else {
-        float co0[8], co1[8], si0[8], si1[8];
-        if constexpr (T32) {
-          const float* cp = static_cast<const float*>(cosT) + int64_t(p) * HD + 8 * ch;
-          const float* sp = static_cast<const float*>(sinT) + int64_t(p) * HD + 8 * ch;
+    if (!rot_ok) {  // a position without an angle: the query is zero, nothing is cached
+      x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
+    } else if (h < nq + c.kv_heads) {
+      uint32_t* a = reinterpret_cast<uint32_t*>(&x0[k]);
+      uint32_t* b = reinterpret_cast<uint32_t*>(&x1[k]);
 #pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            *reinterpret_cast<float4*>(co0 + e) = __ldg(reinterpret_cast<const float4*>(cp + e));
-            *reinterpret_cast<float4*>(co1 + e) = __ldg(reinterpret_cast<const float4*>(cp + HD / 2 + e));
-            *reinterpret_cast<float4*>(si0 + e) = __ldg(reinterpret_cast<const float4*>(sp + e));
-            *reinterpret_cast<float4*>(si1 + e) = __ldg(reinterpret_cast<const float4*>(sp + HD / 2 + e));
-          }
-        } else {
-          const uint16_t* cp = static_cast<const uint16_t*>(cosT) + int64_t(p) * HD + 8 * ch;
-          const uint16_t* sp = static_cast<const uint16_t*>(sinT) + int64_t(p) * HD + 8 * ch;
-          const uint4 a = __ldg(reinterpret_cast<const uint4*>(cp)), b = __ldg(reinterpret_cast<const uint4*>(cp + HD / 2));
-          const uint4 d = __ldg(reinterpret_cast<const uint4*>(sp)), f = __ldg(reinterpret_cast<const uint4*>(sp + HD / 2));
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            *reinterpret_cast<float2*>(co0 + 2 * w) = unpack2<F16>(reinterpret_cast<const uint32_t*>(&a)[w]);
-            *reinterpret_cast<float2*>(co1 + 2 * w) = unpack2<F16>(reinterpret_cast<const uint32_t*>(&b)[w]);
-            *reinterpret_cast<float2*>(si0 + 2 * w) = unpack2<F16>(reinterpret_cast<const uint32_t*>(&d)[w]);
-            *reinterpret_cast<float2*>(si1 + 2 * w) = unpack2<F16>(reinterpret_cast<const uint32_t*>(&f)[w]);
-          }
-        }
-        uint32_t* a = reinterpret_cast<uint32_t*>(&x0);
-        uint32_t* b = reinterpret_cast<uint32_t*>(&x1);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float2 u = unpack2<F16>(a[w]), v = unpack2<F16>(b[w]);
-          a[w] = pack2<F16>(u.x * co0[2 * w] - v.x * si0[2 * w], u.y * co0[2 * w + 1] - v.y * si0[2 * w + 1]);
-          b[w] = pack2<F16>(v.x * co1[2 * w] + u.x * si1[2 * w], v.y * co1[2 * w + 1] + u.y * si1[2 * w + 1]);
-        }
+      for (int w = 0; w < 4; ++w) {
+        const float2 u = unpack2<F16>(a[w]), v = unpack2<F16>(b[w]);
+        a[w] = pack2<F16>(u.x * co0[2 * w] - v.x * si0[2 * w], u.y * co0[2 * w + 1] - v.y * si0[2 * w + 1]);
+        b[w] = pack2<F16>(v.x * co1[2 * w] + u.x * si1[2 * w], v.y * co1[2 * w + 1] + u.y * si1[2 * w + 1]);
       }
     }
-    *reinterpret_cast<uint4*>(dst) = x0;
-    *reinterpret_cast<uint4*>(dst + HD / 2) = x1;
+    *reinterpret_cast<uint4*>(dst) = x0[k];
+    *reinterpret_cast<uint4*>(dst + HD / 2) = x1[k];
   }
 }
 
@@ -1309,16 +1319,19 @@ cudaError_t launch_paged_attn(const PagedCache& c, const PagedAttn& a, const Pag
 cudaError_t launch_paged_append(const PagedCache& c, const uint16_t* qkv, int64_t sqkv, int64_t tokens, const void* cosT,
                                 const void* sinT, bool table32, int max_pos, const int32_t* positions,
                                 const int32_t* slots, const int32_t* seqs, uint16_t* q_out, int nq, cudaStream_t s) {
-  const int threads = std::min(256, (((nq + 2 * c.kv_heads) * c.head_dim / 16) + 31) / 32 * 32);
-  void (*kern)(const PagedCache, const uint16_t*, int64_t, const void*, const void*, int, const int32_t*, const int32_t*,
-               const int32_t*, uint16_t*, int);
+  const int heads = nq + 2 * c.kv_heads, per_token = (heads + kHeads - 1) / kHeads * (c.head_dim / 16);
+  void (*kern)(const PagedCache, const uint16_t*, int64_t, int64_t, const void*, const void*, int, const int32_t*,
+               const int32_t*, const int32_t*, uint16_t*, int, int);
   if (c.head_dim == 64)
     kern = c.f16 ? (table32 ? paged_append_kernel<true, true, 64> : paged_append_kernel<true, false, 64>)
                  : (table32 ? paged_append_kernel<false, true, 64> : paged_append_kernel<false, false, 64>);
   else
     kern = c.f16 ? (table32 ? paged_append_kernel<true, true, 128> : paged_append_kernel<true, false, 128>)
                  : (table32 ? paged_append_kernel<false, true, 128> : paged_append_kernel<false, false, 128>);
-  kern<<<unsigned(tokens), threads, 0, s>>>(c, qkv, sqkv, cosT, sinT, max_pos, positions, slots, seqs, q_out, nq);
+  const int64_t ctas = (tokens * per_token + kAppendThreads - 1) / kAppendThreads;
+  if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+  kern<<<unsigned(ctas), kAppendThreads, 0, s>>>(c, qkv, sqkv, tokens, cosT, sinT, max_pos, positions, slots, seqs, q_out,
+                                                 nq, per_token);
   return cudaGetLastError();
 }
 
