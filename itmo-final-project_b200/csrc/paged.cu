@@ -1188,7 +1188,7 @@ __global__ void __launch_bounds__(256) paged_evict_copy_kernel(const PagedCache 
 #pragma unroll
   for (int k = 0; k < kCopyRows; ++k) {
     from[k] = to[k] = -1;
-    if (pos[k] >= 0) {
+    if (uint32_t(pos[k]) < uint32_t(c.capacity)) {  // (-1 behind the last kept one)
       from[k] = page_entry(c, table, page_of(c, pos[k]));
       to[k] = page_entry(c, new_table + int64_t(b) * new_stride, page_of(c, i0 + k * ROWS));
     }
