@@ -24,6 +24,7 @@ import torch
 from . import _lib
 
 _HALF = (torch.bfloat16, torch.float16)
+_I32, _F32 = torch.int32, torch.float32
 EVICT_MAX_SLOTS = 393216  # I4B_EVICT_MAX_SLOTS
 
 
@@ -43,45 +44,61 @@ def _on_gpu(device: torch.device, *tensors) -> None:
     """Every tensor on the one CUDA device."""
     if device.type != "cuda":
         raise ValueError("int4_b200 computes on the GPU only: the tensors must be CUDA tensors")
+    index = device.index
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"tensors on {t.device} and {device}: one call works on one device")
 
 
 def _indices(t: torch.Tensor, name: str, n: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {n} values")
 
 
 def _table(t: torch.Tensor, name: str) -> None:
-    if t.dtype != torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dtype is not _I32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"{name} must be an int32 tensor [sequences, pages] with unit stride along the pages")
 
 
-def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> bytes:
-    if not (k.dim() == 4 and k.shape == v.shape):
+def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor):
+    """The cache as the C ABI takes it, and (kv_heads, page_size, head_dim, sequences, pages per sequence)."""
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape:
         raise ValueError("k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim]")
-    if not (k.dtype in _HALF and v.dtype == k.dtype):
+    dtype = k.dtype
+    if dtype not in _HALF or v.dtype is not dtype:
         raise ValueError("k_cache and v_cache must both be bfloat16 or both float16")
     _table(table, "block_table")
-    pages, heads, page, dim = k.shape
-    if not (dim in (64, 128)):
+    pages, heads, page, dim = shape
+    if dim not in (64, 128):
         raise ValueError(f"head_dim {dim}: 64 and 128 are supported")
-    if not (page > 0 and page % 8 == 0):
+    if page <= 0 or page % 8:
         raise ValueError(f"page size {page}: a multiple of 8 is needed")
-    ks, vs = k.stride(), v.stride()
-    if not (ks[3] == 1 and vs[3] == 1):
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3 = v.stride()
+    if k3 != 1 or v3 != 1:
         raise ValueError("the caches' last dimension must have unit stride")
     seqs, width = table.shape
-    return _lib.PAGED_CACHE.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.data_ptr(),
-                                 table.stride(0), pages, heads, page, dim, seqs, width, _lib.DTYPE_CODE[k.dtype])
+    return _lib.PAGED_CACHE.pack(k.data_ptr(), v.data_ptr(), k0, k1, k2, v0, v1, v2, table.data_ptr(), table.stride(0),
+                                 pages, heads, page, dim, seqs, width, _lib.DTYPE_CODE[dtype]), heads, page, dim, seqs, width
+
+
+def _accumulator(t: torch.Tensor, B: int, nkv: int, slots: int) -> None:
+    shape = t.shape
+    if t.dtype is not _F32 or len(shape) != 3 or shape[0] != B or shape[1] != nkv or shape[2] < slots \
+            or (shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"weights must be float32 [{B}, {nkv}, at least {slots}] with unit stride along the slots")
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a copy of it if not every row of the last dimension starts on a 16-byte boundary (2-byte elements)."""
-    s = t.stride()
-    if s[-1] == 1 and t.data_ptr() % 16 == 0 and all(x % 8 == 0 or n <= 1 for x, n in zip(s[:-1], t.shape)):
-        return t
+    """``t``, or a copy of it if not every row of the last dimension (a multiple of 64 two-byte elements) starts on a
+    16-byte boundary."""
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        s = t.stride()
+        if s[-1] == 1 and all(x % 8 == 0 or n <= 1 for x, n in zip(s[:-1], t.shape)):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -95,36 +112,36 @@ def paged_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos
     or float32) and goes to slot ``slots[i]`` of sequence ``seqs[i]`` (without ``seqs``: sequence i).  A slot or
     sequence outside ``block_table``, or a page outside the cache, writes nothing (padding); a position outside the
     tables gives a zero query and writes nothing.  Two tokens of a call must not name the same slot of a sequence."""
-    c = _cache(k_cache, v_cache, block_table)
-    nkv, dim = k_cache.shape[1], k_cache.shape[3]
-    if not (qkv.dim() == 2 and qkv.dtype == k_cache.dtype):
+    c, nkv, _, dim, n_seqs, _ = _cache(k_cache, v_cache, block_table)
+    dtype = k_cache.dtype
+    if qkv.dim() != 2 or qkv.dtype is not dtype:
         raise ValueError("qkv must be [tokens, (nq + 2 nkv) * head_dim] of the caches' dtype")
     T, width = qkv.shape
     nq = width // dim - 2 * nkv
     if not (width % dim == 0 and nq > 0):
         raise ValueError(f"qkv rows of {width} values do not hold {nkv} key and value heads of {dim} and queries")
-    if not (cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == dim and cos.shape[0] > 0
-            and cos.dtype == sin.dtype and cos.dtype in (k_cache.dtype, torch.float32) and cos.is_contiguous()
-            and sin.is_contiguous()):
+    angles = cos.shape
+    if not (len(angles) == 2 and angles == sin.shape and angles[1] == dim and angles[0] > 0 and cos.dtype is sin.dtype
+            and (cos.dtype is dtype or cos.dtype is _F32) and cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("cos and sin must be contiguous [max_pos, head_dim], of the caches' dtype or float32")
     _indices(positions, "positions", T)
     _indices(slots, "slots", T)
     if seqs is not None:
         _indices(seqs, "seqs", T)
     else:
-        if not (T <= block_table.shape[0]):
-            raise ValueError(f"{T} tokens without seqs, and a block table of {block_table.shape[0]} sequences")
+        if T > n_seqs:
+            raise ValueError(f"{T} tokens without seqs, and a block table of {n_seqs} sequences")
     if out is None:
         out = qkv.new_empty((T, nq, dim))
     else:
-        if not (out.shape == (T, nq, dim) and out.dtype == qkv.dtype and out.is_contiguous()):
+        if out.shape != (T, nq, dim) or out.dtype is not dtype or not out.is_contiguous():
             raise ValueError("out must be a contiguous [tokens, nq, head_dim] of the caches' dtype")
     dev = qkv.device
     _on_gpu(dev, k_cache, v_cache, block_table, cos, sin, positions, slots, seqs, out)
     qkv = _rows16(qkv)
     with _lib.on_device(dev):
         st = _lib.lib().i4b_paged_kv_append(c, qkv.data_ptr(), qkv.stride(0), T, nq, cos.data_ptr(),
-                                            sin.data_ptr(), _lib.DTYPE_CODE[cos.dtype], cos.shape[0],
+                                            sin.data_ptr(), _lib.DTYPE_CODE[cos.dtype], angles[0],
                                             positions.data_ptr(), slots.data_ptr(),
                                             None if seqs is None else seqs.data_ptr(), out.data_ptr(),
                                             _lib.stream_handle(dev))
@@ -141,23 +158,20 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     ``scale`` is head_dim ** -0.5 unless given.  ``weights`` (float32 ``[B, nkv, >= pages * page_size]``) is added to
     in place: slot j of a sequence gets its probability summed over the query heads of the kv head, which is what
     ``paged_evict`` selects by.  Lengths are clamped to what the block table's rows can hold."""
-    c = _cache(k_cache, v_cache, block_table)
-    nkv, page, dim = k_cache.shape[1:]
-    B, width = block_table.shape
-    if not (q.dim() == 3 and q.shape[0] == B and q.shape[2] == dim and q.dtype == k_cache.dtype):
+    c, nkv, page, dim, B, width = _cache(k_cache, v_cache, block_table)
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != dim or q.dtype is not k_cache.dtype:
         raise ValueError("q must be [sequences, nq, head_dim] of the caches' dtype")
-    nq = q.shape[1]
-    if not (nq > 0 and nq % nkv == 0):
+    nq = shape[1]
+    if nq <= 0 or nq % nkv:
         raise ValueError(f"{nq} query heads do not divide over {nkv} kv heads")
     _indices(lens, "lens", B)
     if weights is not None:
-        if not (weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
-                and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1)):
-            raise ValueError(f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
+        _accumulator(weights, B, nkv, width * page)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        if not (out.shape == (B, nq, dim) and out.dtype == q.dtype and out.is_contiguous()):
+        if out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous():
             raise ValueError("out must be a contiguous [sequences, nq, head_dim] of the caches' dtype")
     dev = q.device
     _on_gpu(dev, k_cache, v_cache, block_table, lens, weights, out)
@@ -166,12 +180,11 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     # from torch's allocator each time: two captured graphs never share it, and eager streams do not either
     ws = lens.new_empty(need, dtype=torch.uint8) if need else None
     with _lib.on_device(dev):
-        st = _lib.lib().i4b_paged_decode_attention(c, q.data_ptr(), q.stride(0), q.stride(1), nq, lens.data_ptr(),
-                                          dim ** -0.5 if scale is None else scale, out.data_ptr(),
-                                          None if weights is None else weights.data_ptr(),
-                                          0 if weights is None else weights.stride(0),
-                                          0 if weights is None else weights.stride(1), None if ws is None else ws.data_ptr(), need,
-                                          _lib.stream_handle(dev))
+        st = _lib.lib().i4b_paged_decode_attention(
+            c, q.data_ptr(), q.stride(0), q.stride(1), nq, lens.data_ptr(), dim ** -0.5 if scale is None else scale,
+            out.data_ptr(), None if weights is None else weights.data_ptr(),
+            0 if weights is None else weights.stride(0), 0 if weights is None else weights.stride(1),
+            None if ws is None else ws.data_ptr(), need, _lib.stream_handle(dev))
     _lib.check(st, "paged_decode_attention")
     return out
 
@@ -187,12 +200,8 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
     all of them.  The new pages must not be pages that this call reads.  Returns ``(new_lens[B], kept[B, nkv, budget],
     weights_out[B, nkv, W])``: the lengths afterwards, the slots kept (-1 behind the last one) and their weights (zeros
     behind the last; ``weights_out`` may be ``weights`` itself)."""
-    c = _cache(k_cache, v_cache, block_table)
-    nkv, page = k_cache.shape[1:3]
-    B, width = block_table.shape
-    if not (weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, nkv)
-            and weights.shape[2] >= width * page and (weights.shape[2] <= 1 or weights.stride(2) == 1)):
-        raise ValueError(f"weights must be float32 [{B}, {nkv}, at least {width * page}] with unit stride along the slots")
+    c, nkv, page, _, B, width = _cache(k_cache, v_cache, block_table)
+    _accumulator(weights, B, nkv, width * page)
     if not (width * page <= EVICT_MAX_SLOTS):
         raise ValueError(f"{width * page} slots per sequence: eviction selects from at most {EVICT_MAX_SLOTS}")
     _indices(lens, "lens", B)
