@@ -314,7 +314,7 @@ typedef struct i4b_paged_cache {
  * receives the rotated queries.  t * cos + rotate_half(t) * sin is computed in fp32 and rounded once
  * (i4b_rope_kv_cache rounds each product too, as transformers does).  A slot or sequence outside the table writes
  * nothing to the cache (padding); a position outside the tables gives a zero query and writes nothing.  Two tokens of
- * one call must not name the same slot of the same sequence. */
+ * one call must not name the same slot of the same sequence, nor slots of two sequences that share the page. */
 int i4b_paged_kv_append(const i4b_paged_cache* cache, const void* qkv, int64_t stride_qkv, int64_t tokens, int64_t nq,
                         const void* cos_table, const void* sin_table, int table_dtype, int64_t max_pos,
                         const int32_t* positions, const int32_t* slots, const int32_t* seqs, void* q_out, void* stream);
@@ -343,7 +343,7 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
  * page_size rounded up] names the new pages, none of which may be a page that `cache` still reads in this call.
  * new_lens[seqs] = min(lens, budget); kept[seqs, kv_heads, budget] (contiguous) = the slots kept, -1 behind the last;
  * weights_out [seqs, kv_heads, width] = their weights, zeros behind the last (may be `weights` itself).
- * 0 <= recent <= budget, budget >= 1; max_pages * page_size <= I4B_EVICT_MAX_SLOTS. */
+ * 0 <= recent <= budget, 1 <= budget <= 2^30, width <= 2^30; max_pages * page_size <= I4B_EVICT_MAX_SLOTS. */
 #define I4B_EVICT_MAX_SLOTS 393216
 int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t stride_wb, int64_t stride_wh,
                     int64_t width, const int32_t* lens, const int32_t* new_table, int64_t new_table_stride,
@@ -351,7 +351,7 @@ int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t 
                     float* weights_out, int64_t stride_ob, int64_t stride_oh, void* stream);
 
 /* Log probabilities of given tokens, with each row's entropy and most probable tokens, in one reading of the logits.
- * x: row r at x + r * stride_x, n contiguous logits of dtype I4B_BF16, I4B_F16 or I4B_F32.
+ * x: row r at x + r * stride_x, n <= 2^30 contiguous logits of dtype I4B_BF16, I4B_F16 or I4B_F32.
  * logprobs[r] = x[r, targets[r]] - logsumexp(x[r]); a negative target (padding) gives 0, one >= n a NaN.
  * entropy[r] = -sum p log p.  top_ids / top_logprobs [rows, top]: the `top` largest logits of the row in order, ties to
  * the lower index, with their log probabilities (0 <= top <= I4B_MAX_TOP, top <= n; both may be NULL when top is 0).

@@ -658,7 +658,7 @@ int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t 
                     float* weights_out, int64_t stride_ob, int64_t stride_oh, void* stream) {
   PagedCache c;
   if (int st = paged_cache(cache, &c)) return st;
-  if (c.capacity > paged_evict_most() || width < c.capacity || width > INT32_MAX - 64 || budget < 1 || budget > INT32_MAX - 64 || recent < 0 ||
+  if (c.capacity > paged_evict_most() || width < c.capacity || width > (1 << 30) || budget < 1 || budget > (1 << 30) || recent < 0 ||
       recent > budget || new_max_pages < (budget + c.page_size - 1) / c.page_size)
     return I4B_ERR_SHAPE;
   if (c.seqs == 0) return I4B_OK;
@@ -675,7 +675,7 @@ int i4b_token_logprobs(const void* x, int dtype, int64_t rows, int64_t n, int64_
                        int64_t top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
                        void* stream) {
   if (dtype != I4B_BF16 && dtype != I4B_F16 && dtype != I4B_F32) return I4B_ERR_INVALID_ARG;
-  if (rows < 0 || rows > INT32_MAX || n <= 0 || n > INT32_MAX - 64 || stride_x < 0 || top < 0 || top > I4B_MAX_TOP ||
+  if (rows < 0 || rows > INT32_MAX || n <= 0 || n > (1 << 30) || stride_x < 0 || top < 0 || top > I4B_MAX_TOP ||
       top > n)
     return I4B_ERR_SHAPE;
   if (rows == 0) return I4B_OK;

@@ -568,8 +568,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
           for (int e = 0; e < 2; ++e)
             if (KI * e + i >= there) s[r][i][2 * e] = s[r][i][2 * e + 1] = -INFINITY;
     }
-    // The reference point m of the exponentials follows the maximum with a slack of 2^8: it moves, and what is summed
-    // so far is scaled, only when a score passes it by more (and with a head's first score).
+    // The running maximum m: only when a score of the tile passes it (the lanes vote) is it found over the lanes, and
+    // what is summed so far scaled.  No probability exceeds 1.
     bool grew = false;
     float mx[R][2];
 #pragma unroll
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
         mx[r][u] = fmaxf(s[r][0][u], s[r][0][2 + u]);
 #pragma unroll
         for (int i = 1; i < KI; ++i) mx[r][u] = fmaxf(mx[r][u], fmaxf(s[r][i][u], s[r][i][2 + u]));
-        grew |= fmaf(mx[r][u], scl, -8.0f) > m[r][u];
+        grew |= mx[r][u] * scl > m[r][u];
       }
     if (__any_sync(0xFFFFFFFFu, grew)) {
 #pragma unroll

@@ -88,6 +88,8 @@ def _accumulator(t: torch.Tensor, B: int, nkv: int, slots: int) -> None:
     if t.dtype is not _F32 or len(shape) != 3 or shape[0] != B or shape[1] != nkv or shape[2] < slots \
             or (shape[2] > 1 and t.stride(2) != 1):
         raise ValueError(f"weights must be float32 [{B}, {nkv}, at least {slots}] with unit stride along the slots")
+    if (B > 1 and t.stride(0) == 0) or (nkv > 1 and t.stride(1) == 0):
+        raise ValueError("weights of different sequences or kv heads must not be the same memory")
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -286,7 +288,7 @@ class PagedKVCache:
 
     def reserve_step(self) -> None:
         """Host side of a decode step: a slot for every live sequence (before the step, or before its graph replays)."""
-        live = [seq for seq in range(self.max_seqs) if self.pages[seq]]
+        live = [seq for seq in range(self.max_seqs) if self.lengths[seq] > 0]
         self.reserve({seq: 1 for seq in live})
         for seq in live:
             self.lengths[seq] += 1

@@ -44,6 +44,8 @@ def test_attention_refuses_weights_and_out_of_other_shapes():
     for w in (s["weights"][:, :, :-1], s["weights"][:, :1], s["weights"].double(), s["weights"].transpose(1, 2)):
         with pytest.raises(ValueError, match="weights"):
             _attend(s, weights=w)
+    with pytest.raises(ValueError, match="same memory"):
+        _attend(s, weights=s["weights"][:1].expand(2, 2, 48))
     for out in (torch.zeros(2, 8, 64), torch.zeros(2, 8, 128, dtype=torch.bfloat16)[..., :64]):
         with pytest.raises(ValueError, match="out must be"):
             _attend(s, out=out)
@@ -114,6 +116,7 @@ def test_c_attention_statuses(change, status):
 
 def test_c_statuses_of_the_other_arguments():
     L = _lib.lib()
+    assert _c_attend(_struct(kv_heads=1), nq=1025) == 2  # query heads per kv head
     assert _c_attend(_struct(), nq=7) == 2 and _c_attend(_struct(), q=None) == 1 and _c_attend(_struct(), q=0x4008) == 4
     assert _c_attend(_struct(seqs=0)) == 0  # nothing to do
     assert _c_attend(_struct(kv_heads=1, k_stride_head=3, v_stride_head=5), q=None) == 1  # a stride that is never used
@@ -130,12 +133,13 @@ def test_c_statuses_of_the_other_arguments():
         return L.i4b_paged_evict(c, weights, 96, 48, width, 0x5000, 0x5100, 2, new_pages, budget, recent, 0x6000, 0x6100,
                                  0x6200, 96, 48, None)
 
-    assert evict(width=47) == 2 and evict(new_pages=1) == 2 and evict(budget=0) == 2 and evict(recent=33) == 2 and evict(weights=None) == 1
+    assert evict(width=47) == 2 and evict(width=(1 << 30) + 1) == 2 and evict(budget=(1 << 30) + 1, new_pages=1 << 30) == 2
+    assert evict(new_pages=1) == 2 and evict(budget=0) == 2 and evict(recent=33) == 2 and evict(weights=None) == 1
 
     def logprobs(dtype=1, rows=2, n=100, stride=100, top=0, x=0x4000, ids=None):
         return L.i4b_token_logprobs(x, dtype, rows, n, stride, 0x5000, top, 0x6000, 0x6100, 0x6200, ids, None)
 
-    assert logprobs(dtype=3) == 1 and logprobs(n=0) == 2 and logprobs(top=33) == 2 and logprobs(n=4, top=5) == 2 and logprobs(rows=-1) == 2
+    assert logprobs(dtype=3) == 1 and logprobs(n=(1 << 30) + 1) == 2 and logprobs(n=0) == 2 and logprobs(top=33) == 2 and logprobs(n=4, top=5) == 2 and logprobs(rows=-1) == 2
     assert logprobs(x=None) == 1 and logprobs(top=3) == 1 and logprobs(x=0x4001) == 4 and logprobs(rows=0) == 0
 
 

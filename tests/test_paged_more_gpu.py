@@ -171,3 +171,57 @@ def test_logprobs_on_two_streams_at_once(cuda_device):
             got += [int4_b200.token_logprobs(z, t, top=7) for _ in range(5)]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_scores_that_grow_and_shrink(cuda_device, dtype):
+    """Scores that rise by hundreds along the sequence, fall, or are all alike; values near the type's range; a negative scale."""
+    import int4_b200
+
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    n, dim, page = 700, 64, 16
+    pages = -(-n // page)
+    for kind in ("rising", "falling", "flat", "steps"):
+        ramp = {"rising": torch.arange(n) * 0.5, "falling": -torch.arange(n) * 0.5, "flat": torch.zeros(n),
+                "steps": (torch.arange(n) // 64 % 3) * 6.0}[kind].cuda()
+        kk = torch.randn(n, dim, device="cuda", generator=gen)
+        kk[:, 0] = ramp
+        q = torch.randn(1, 4, dim, device="cuda", generator=gen)
+        q[..., 0] = 4.0
+        q = q.to(dtype)
+        big = 1e36 if dtype == torch.bfloat16 else 6e4
+        v0 = torch.rand(n, dim, device="cuda", generator=gen) * big
+        k = torch.zeros(pages, 1, page, dim, device="cuda", dtype=dtype)
+        v = torch.zeros_like(k)
+        k.view(-1, dim)[:n], v.view(-1, dim)[:n] = kk.to(dtype), v0.to(dtype)
+        table = torch.arange(pages, device="cuda", dtype=torch.int32)[None]
+        lens = torch.tensor([n], device="cuda", dtype=torch.int32)
+        for scale in (0.125, -0.125, 1.0):
+            w = torch.zeros(1, 1, pages * page, device="cuda")
+            out = int4_b200.paged_decode_attention(q, k, v, table, lens, scale=scale, weights=w)
+            kd, vd = k.view(-1, dim)[:n].double(), v.view(-1, dim)[:n].double()
+            s = q[0].double() @ kd.T * scale
+            p = torch.softmax(s, -1)
+            # fp32 scores: 64 products and sums, the scale and the subtraction, at the size of the largest
+            eps = (dim + 8) * 2 ** -24 * float((q[0].double().abs() @ kd.abs().T).max()) * abs(scale) * 2 + 2 ** -20
+            half = torch.finfo(dtype).eps / 2
+            ref = p @ vd
+            # fp16 holds a probability as two numbers down to 2^-24 of the range's top: n of them, each off by 2^-25 at most
+            small = n * 2 ** -25 * float(vd.max()) * (1 if dtype == torch.float16 else 0)
+            assert torch.isfinite(out).all()
+            assert ((out[0].double() - ref).abs() <= half * ref + 2 * eps * ref + small).all(), (kind, scale)
+            assert ((w[0, 0, :n].double() - p.sum(0)).abs() <= p.sum(0) * (2 * eps + 2 ** -20) + 2 ** -60).all(), (kind, scale)
+
+
+def test_attention_output_may_take_the_queries_place(cuda_device):
+    import int4_b200
+
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    for cap in (12, 300):
+        k = torch.randn(cap * 2, 2, 16, 64, device="cuda", generator=gen).bfloat16()
+        v = torch.randn(cap * 2, 2, 16, 64, device="cuda", generator=gen).bfloat16()
+        table = torch.arange(cap * 2, device="cuda", dtype=torch.int32).view(2, cap)
+        lens = torch.tensor([cap * 16, cap * 16 - 37], device="cuda", dtype=torch.int32)
+        q = torch.randn(2, 8, 64, device="cuda", generator=gen).bfloat16()
+        want = int4_b200.paged_decode_attention(q, k, v, table, lens)
+        assert torch.equal(int4_b200.paged_decode_attention(q, k, v, table, lens, out=q), want)
