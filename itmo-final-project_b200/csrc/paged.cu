@@ -192,7 +192,7 @@ constexpr int kAttnWarps = 5;
 constexpr int kAttnCtas = 2;
 constexpr int kUnit = 4096;  // bytes of a tile's keys, or values
 constexpr int kUnits = 4;    // in flight per warp: keys and values of two tiles
-constexpr int kMinTiles = 2;
+constexpr int kMinTiles = 1;
 
 __host__ __device__ constexpr int attn_warp_smem(int head_dim, bool two) { return kUnits * kUnit + (two ? 2 : 1) * head_dim * 16; }
 
@@ -836,7 +836,9 @@ __device__ __forceinline__ void join_head(const JoinArgs& g, int64_t at, int tid
   *reinterpret_cast<uint2*>(dst + 4 * x) = make_uint2(pack2<F16>(a.x * inv, a.y * inv), pack2<F16>(a.z * inv, a.w * inv));
 }
 
-// TPH = 32 from 2048 heads on (8 of them in a CTA), 128 from 512 on, else 512 (one each).
+// TPH (a whole attention call in a captured loop): 32, eight heads in a CTA, from 2048 heads on, or from 512 where the
+// tables hold at most 128 tiles (32 sequences up to 2047: 21.3 us, with 128 24.1; 24 up to 8191 at head_dim 128, 1536
+// heads of some 40 pieces: 102.4, with 128 99.4); else 128 from 512 heads on or with such tables, else 512.
 template <bool F16, int HD, int TPH>
 __global__ void __launch_bounds__(TPH == 32 ? 256 : TPH) paged_attn_join_kernel(const JoinArgs g) {
   const int64_t at = TPH == 32 ? int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
@@ -1257,9 +1259,11 @@ cudaError_t attn(const PagedCache& c, const PagedAttn& a, const PagedAttnWorkspa
                         dim3(unsigned(joins + items * wa.parts)), dim3(256), 0, s, c, a.lens, g, joins, wa);
   }
   if (whole) return cudaSuccess;
-  if (heads >= 2048)
+  const bool few = c.capacity <= 128 * tile_of(HD);  // pieces per head: at most 128
+  if (heads >= (few ? 512 : 2048))
     return launch_after(paged_attn_join_kernel<F16, HD, 32>, dim3(unsigned((heads + 7) / 8)), dim3(256), 0, s, g);
-  if (heads >= 512) return launch_after(paged_attn_join_kernel<F16, HD, 128>, dim3(unsigned(heads)), dim3(128), 0, s, g);
+  if (few || heads >= 512)
+    return launch_after(paged_attn_join_kernel<F16, HD, 128>, dim3(unsigned(heads)), dim3(128), 0, s, g);
   return launch_after(paged_attn_join_kernel<F16, HD, 512>, dim3(unsigned(heads)), dim3(512), 0, s, g);
 }
 
