@@ -133,8 +133,9 @@ __device__ __forceinline__ Stat merge(const Stat& x, const Stat& y) {
 
 // N chunks at once: their maximum first, then, in units of log 2, t = z log2(e) - m log2(e) in one packed operation of
 // two elements, as are the two sums: 3.75 instructions per element.  m log2(e) is rounded, off by delta, and with it
-// every t: the sums are put right for that afterwards.  A -inf, a NaN or a +inf among the logits, or one so large that t
-// overflows, leaves no finite sum; such a batch is taken again one by one.
+// every t: the sums are put right for that afterwards, while |delta| <= 1 (|m| <= 2^24; beyond, 2^delta could leave
+// fp32's range).  A -inf, a NaN or a +inf among the logits, or one so large that t overflows, leaves no finite sum; such
+// a batch, and one of a larger m, is taken again one by one.
 template <typename E, int N>
 __device__ __forceinline__ void add_batch(Stat& st, const uint4 (&w)[N]) {
   float top = E::most(w[0]);
@@ -159,8 +160,8 @@ __device__ __forceinline__ void add_batch(Stat& st, const uint4 (&w)[N]) {
   }
   const float2 s = unpack(s2), a = unpack(a2);
   const float ss = s.x + s.y, as = a.x + a.y;
-  if (as - as == 0.0f) {  // finite
-    const float back = 1.0f - delta * kLn2;  // 2^-delta
+  if (as - as == 0.0f && fabsf(st.m) <= 16777216.0f) {  // (the difference: finite)
+    const float back = ex2(-delta);
     st.s = fmaf(ss, back, st.s);
     st.a = fmaf((as - delta * ss) * kLn2, back, st.a);
   } else {

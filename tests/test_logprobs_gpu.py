@@ -141,3 +141,33 @@ def test_captured_and_replayed(cuda_device):
         g.replay()
         want = int4_b200.token_logprobs(z2, t2, top=5)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("rows", [2, 300])
+@pytest.mark.parametrize("m", [1.0e3, 1.2345e5, 1.0e6, 12345678.0, 2.0 ** 40, 3.3e9, 1.1e20, 2.5e38])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_logits(cuda_device, dtype, m, rows):
+    """k tokens share the largest logit, +m or -m, the others are far below: log probabilities -log k, entropy log k.
+
+    Each of the k terms and the factor that puts a row's maximum right is an exponential of an argument up to 1 (off by
+    2^-22 relatively); k <= 24 terms add at most 24 half steps, the products, quotients and the logarithm a few more:
+    2^-21 + 40 * 2^-24 < 2^-18 with log 24 < 4."""
+    import int4_b200
+
+    n, k = 6001, [1, 2, 7, 24]
+    gen = torch.Generator().manual_seed(int(math.log2(m)))
+    z = torch.empty(rows, n, dtype=torch.float32)
+    picked = []
+    for r in range(rows):
+        sign = 1.0 if r % 2 == 0 else -1.0
+        z[r] = {0: -math.inf, 1: torch.finfo(dtype).min, 2: sign * m - 0.2 * m}[r // 2 % 3]
+        at = torch.randperm(n, generator=gen)[: k[r % 4]].sort().values
+        z[r, at] = sign * m
+        picked.append(at)
+    t = torch.tensor([int(at[-1]) for at in picked], device="cuda")
+    lp, entropy, top_lp, top_ids = int4_b200.token_logprobs(z.to(dtype).cuda(), t, top=1)
+    want = torch.tensor([math.log(len(at)) for at in picked], dtype=torch.float64)
+    assert ((lp.cpu().double() + want).abs() <= 2.0 ** -18).all(), lp.cpu().double() + want
+    assert ((top_lp[:, 0].cpu().double() + want).abs() <= 2.0 ** -18).all()
+    assert ((entropy.cpu().double() - want).abs() <= 2.0 ** -18).all(), entropy.cpu().double() - want
+    assert top_ids[:, 0].cpu().tolist() == [int(at[0]) for at in picked]
