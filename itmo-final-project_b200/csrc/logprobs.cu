@@ -131,18 +131,27 @@ __device__ __forceinline__ Stat merge(const Stat& x, const Stat& y) {
   return r;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // N chunks at once: their maximum first, then, in units of log 2, t = z log2(e) - m log2(e) in one packed operation of
-// two elements, as are the two sums: 3.75 instructions per element.  m log2(e) is rounded, off by delta, and with it
+// two elements, as are the two sums: 4.75 instructions per element.  m log2(e) is rounded, off by delta, and with it
 // every t: the sums are put right for that afterwards, while |delta| <= 1 (|m| <= 2^24; beyond, 2^delta could leave
-// fp32's range).  A -inf, a NaN or a +inf among the logits, or one so large that t overflows, leaves no finite sum; such
-// a batch, and one of a larger m, is taken again one by one.
+// fp32's range).  Every logit is first raised to m - 200 (e^-200 is 0 in fp32, its terms stay 0): a mask's -inf or lowest
+// value would make 0 * inf.  Without that, masked batches had to go one by one: 198 instead of 90 us for 2048 x 128256
+// bf16 with any -inf in each batch, 19.3 instead of 15.1 for 61 x 100003 fp32, against 88 instead of 90 where nothing is
+// masked.  A NaN or a +inf leaves no finite sum; such a batch, and one of a larger |m|, is taken again one by one.
 template <typename E, int N>
 __device__ __forceinline__ void add_batch(Stat& st, const uint4 (&w)[N]) {
   float top = E::most(w[0]);
 #pragma unroll
   for (int u = 1; u < N; ++u) top = fmaxf(top, E::most(w[u]));
   if (top > st.m) raise(st, top);
-  const float ml = st.m * kLog2e, delta = fmaf(st.m, kLog2e, -ml);
+  const float m = st.m == -INFINITY ? 0.0f : st.m, low = m - 200.0f;  // (nothing but masked ones so far: all sums 0)
+  const float ml = m * kLog2e, delta = fmaf(m, kLog2e, -ml);
   const uint64_t nm = pack(-ml, -ml), l2 = pack(kLog2e, kLog2e);
   uint64_t s2 = 0, a2 = 0;
 #pragma unroll
@@ -151,7 +160,7 @@ __device__ __forceinline__ void add_batch(Stat& st, const uint4 (&w)[N]) {
     E::many(w[u], f);
 #pragma unroll
     for (int i = 0; i < E::kVec; i += 2) {
-      const uint64_t t2 = fma2(pack(f[i], f[i + 1]), l2, nm);
+      const uint64_t t2 = fma2(pack(max_nan(f[i], low), max_nan(f[i + 1], low)), l2, nm);
       const float2 t = unpack(t2);
       const uint64_t e = pack(ex2(t.x), ex2(t.y));
       s2 = add2(s2, e);
@@ -160,7 +169,7 @@ __device__ __forceinline__ void add_batch(Stat& st, const uint4 (&w)[N]) {
   }
   const float2 s = unpack(s2), a = unpack(a2);
   const float ss = s.x + s.y, as = a.x + a.y;
-  if (as - as == 0.0f && fabsf(st.m) <= 16777216.0f) {  // (the difference: finite)
+  if (as - as == 0.0f && fabsf(m) <= 16777216.0f) {  // (the difference: finite)
     const float back = ex2(-delta);
     st.s = fmaf(ss, back, st.s);
     st.a = fmaf((as - delta * ss) * kLn2, back, st.a);
