@@ -633,7 +633,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float x0 = s[r][i][2 * e], x1 = s[r][i][2 * e + 1];
-          float p0 = ex2(fmaf(x0, scl, n0)), p1 = ex2(fmaf(x1, scl, n1));
+          // rounded before the difference, as m and the stored scores are: the largest is exactly 2^0 however large it is
+          float p0 = ex2(__fadd_rn(__fmul_rn(x0, scl), n0)), p1 = ex2(__fadd_rn(__fmul_rn(x1, scl), n1));
           if (!(f & 1u)) {  // (a scale of 0 would make a NaN of a place that is not there)
             p0 = x0 == -INFINITY ? 0.0f : p0;
             p1 = x1 == -INFINITY ? 0.0f : p1;

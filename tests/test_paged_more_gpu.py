@@ -225,3 +225,33 @@ def test_attention_output_may_take_the_queries_place(cuda_device):
         q = torch.randn(2, 8, 64, device="cuda", generator=gen).bfloat16()
         want = int4_b200.paged_decode_attention(q, k, v, table, lens)
         assert torch.equal(int4_b200.paged_decode_attention(q, k, v, table, lens, out=q), want)
+
+
+@pytest.mark.parametrize("cap_pages", [3, 80])  # whole items; split runs
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 30.0), (torch.bfloat16, 3.3e3), (torch.bfloat16, 1e9), (torch.float16, 1.7e3),
+                                        (torch.float16, 6e4)])
+def test_attention_of_large_scores(cuda_device, dtype, size, cap_pages):
+    """One slot's score, or two equal ones, far above all others: probabilities of 1, or of 1/2 each, at any size of the
+    scores; the others' are 0 (the smallest distance is 64 * 30 * 30 * 0.125 / 2 = 3600).  All of this is exact."""
+    import int4_b200
+
+    B, nkv, G, dim, ps = 3, 2, 4, 64, 16
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    pages = B * cap_pages
+    k = torch.full((pages, nkv, ps, dim), -size, device="cuda").to(dtype)
+    v = torch.randn(pages, nkv, ps, dim, device="cuda", generator=gen).to(dtype)
+    table = torch.randperm(pages, device="cuda", generator=gen).int().view(B, cap_pages)
+    lens = torch.tensor([cap_pages * ps, cap_pages * ps - 5, 37], device="cuda", dtype=torch.int32)
+    q = torch.full((B, nkv * G, dim), size, device="cuda").to(dtype)
+    w = torch.zeros(B, nkv, cap_pages * ps, device="cuda")
+    want_w, want = w.clone(), torch.empty(B, nkv, dim, device="cuda")
+    for b in range(B):
+        for h in range(nkv):
+            at = [7, 36] if h else [int(lens[b]) - 3]
+            for j in at:
+                k[table[b, j // ps].long(), h, j % ps] = torch.tensor(size / 2).to(dtype)
+                want_w[b, h, j] = G / len(at)
+            want[b, h] = sum(v[table[b, j // ps].long(), h, j % ps].float() for j in at) / len(at)
+    out = int4_b200.paged_decode_attention(q, k, v, table, lens, weights=w)
+    assert torch.equal(out, want.to(dtype).repeat_interleave(G, dim=1))
+    assert torch.equal(w, want_w)
