@@ -194,6 +194,15 @@ constexpr int kUnit = 4096;  // bytes of a tile's keys, or values
 constexpr int kUnits = 4;    // in flight per warp: keys and values of two tiles
 constexpr int kMinTiles = 1;
 
+// The probabilities enter the second product as the sum of two values of the cache's type, the rounded one and what that
+// leaves; rounded once, they would be off as much as the output's own rounding is.  bf16 has fp32's exponents, both go
+// into one sum.  fp16 ends at 2^-24: probabilities of 0 to 1 would lose what lies 17 below a row's largest score, all of
+// the output where that slot's value is 0.  They are multiplied by 2^15 (1 becomes 32768), the rest, at most 8 there, by
+// 2^11 once more and taken into a product of its own, added with 2^-11 for each tile: every probability within 2^-22 of
+// itself, or within 2^-51.  (A second sum over the tiles would spill: the kernel is at its 168 registers.)  The factors
+// are powers of two and leave the output before anything else sees it, so they round nothing.
+constexpr float kP16 = 32768.0f, kRest16 = 2048.0f;
+
 __host__ __device__ constexpr int attn_warp_smem(int head_dim, bool two) { return kUnits * kUnit + (two ? 2 : 1) * head_dim * 16; }
 
 __host__ __device__ constexpr int tile_of(int head_dim) { return kUnit / 2 / head_dim; }  // 32 or 16 positions
@@ -622,8 +631,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
             }
           }
     }
-    // probabilities, for the second product as the sum of two values of the cache's type (the rounded one and what that
-    // leaves): rounded once, they would be off as much as the output's own rounding is
+    // probabilities, each as two values of the cache's type
     uint32_t pb[R][KI][2], pc[R][KI][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -640,10 +648,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
             p1 = x1 == -INFINITY ? 0.0f : p1;
           }
           l[r][0] += p0, l[r][1] += p1;
+          if constexpr (F16) p0 *= kP16, p1 *= kP16;
           const uint32_t w = pack2<F16>(p0, p1);
           const float2 back = unpack2<F16>(w);
           pb[r][i][e] = transpose8(w);
-          pc[r][i][e] = transpose8(pack2<F16>(p0 - back.x, p1 - back.y));
+          const float u = F16 ? kRest16 : 1.0f;
+          pc[r][i][e] = transpose8(pack2<F16>((p0 - back.x) * u, (p1 - back.y) * u));
         }
     }
     // ---- output: dims 8(g + 8v) + 2w and + 2w + 1 are rows g and g + 8 of block 4v + w
@@ -652,7 +662,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
     {
       const uint4* src = ring + (2 + (n & 1)) * kSlot + 8 * t + (g ^ (2 * t));
 #pragma unroll
-      for (int v = 0; v < VC; ++v)
+      for (int v = 0; v < VC; ++v) {
+        float rest[R][4][4];
 #pragma unroll
         for (int i = 0; i < KI; ++i) {
           const uint4 a = src[(i * VC + v) * 32], b = src[((KR + i) * VC + v) * 32];
@@ -666,10 +677,24 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
 #pragma unroll
             for (int r = 0; r < R; ++r) {
               mma_16816<F16>(o[r][4 * v + w], va, pb[r][i][0], pb[r][i][1]);
-              mma_16816<F16>(o[r][4 * v + w], va, pc[r][i][0], pc[r][i][1]);
+              if constexpr (!F16)
+                mma_16816<F16>(o[r][4 * v + w], va, pc[r][i][0], pc[r][i][1]);
+              else if (i == 0)
+                mma_16816_first<F16>(rest[r][w], va, pc[r][i][0], pc[r][i][1]);
+              else
+                mma_16816<F16>(rest[r][w], va, pc[r][i][0], pc[r][i][1]);
             }
           }
         }
+        if constexpr (F16) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[r][4 * v + w][j] = fmaf(rest[r][w][j], 1.0f / kRest16, o[r][4 * v + w][j]);
+        }
+      }
     }
     request_values(ring + (2 + (n & 1)) * kSlot, n + 2);
     fetch_page();
@@ -679,6 +704,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kAttnCtas)
       const int kvh = HT == 1 ? ci.h : ci.h / HT, head0 = kvh * G + (HT == 1 ? 0 : ci.h % HT) * 16;
       const int rows = min(16, kvh * G + G - head0);
       const bool whole = seg_tile0 == 0 && ctile == ci.nt - 1;
+      if constexpr (F16) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < 4 * VC; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[r][i][j] *= 1.0f / kP16;
+      }
       float* part = partials + int64_t(2 * run + (first_seg ? 0 : 1)) * piece;
 #pragma unroll
       for (int r = 0; r < R; ++r)
