@@ -342,7 +342,8 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
  * weights: fp32 [seqs, kv_heads, width] with strides, width >= max_pages * page_size.  new_table[seqs, >= budget /
  * page_size rounded up] names the new pages, none of which may be a page that `cache` still reads in this call.
  * new_lens[seqs] = min(lens, budget); kept[seqs, kv_heads, budget] (contiguous) = the slots kept, -1 behind the last;
- * weights_out [seqs, kv_heads, width] = their weights, zeros behind the last (may be `weights` itself).
+ * weights_out [seqs, kv_heads, width] = their weights, zeros behind the last (may be `weights` itself; otherwise no two
+ * of its rows, nor one of its rows and one of weights, may have memory in common).
  * 0 <= recent <= budget, 1 <= budget <= 2^30, width <= 2^30; max_pages * page_size <= I4B_EVICT_MAX_SLOTS. */
 #define I4B_EVICT_MAX_SLOTS 393216
 int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t stride_wb, int64_t stride_wh,

@@ -590,6 +590,11 @@ int paged_cache(const i4b_paged_cache* in, PagedCache* c) {
   return I4B_OK;
 }
 
+// Rows of n values that are written, by different CTAs, where the next sequence's or kv head's are.
+bool rows_meet(const PagedCache& c, int64_t stride_b, int64_t stride_h, int64_t n) {
+  return (c.seqs > 1 && stride_b < n && stride_b > -n) || (c.kv_heads > 1 && stride_h < n && stride_h > -n);
+}
+
 }  // namespace
 
 int i4b_paged_kv_append(const i4b_paged_cache* cache, const void* qkv, int64_t stride_qkv, int64_t tokens, int64_t nq,
@@ -663,6 +668,7 @@ int i4b_paged_evict(const i4b_paged_cache* cache, const float* weights, int64_t 
     return I4B_ERR_SHAPE;
   if (c.seqs == 0) return I4B_OK;
   if (!lens || !new_table || !new_lens || !kept || (width > 0 && (!weights || !weights_out))) return I4B_ERR_INVALID_ARG;
+  if (rows_meet(c, stride_ob, stride_oh, width)) return I4B_ERR_LAYOUT;
   DevInfo d;
   if (int st = current_device_info(&d)) return st;
   const PagedEvict p = {weights, stride_wb, stride_wh, lens, new_table, new_table_stride, int(budget), int(recent),

@@ -92,6 +92,34 @@ def _accumulator(t: torch.Tensor, B: int, nkv: int, slots: int) -> None:
         raise ValueError("weights of different sequences or kv heads must not be the same memory")
 
 
+def _starts(t: torch.Tensor) -> torch.Tensor:
+    """Where the rows t[b, h] begin in memory, in elements of 4 bytes, in order."""
+    (B, nkv), (s0, s1) = t.shape[:2], t.stride()[:2]
+    at = torch.arange(B)[:, None] * s0 + torch.arange(nkv) * s1 + t.data_ptr() // 4
+    return at.flatten().sort().values
+
+
+def _rows_meet(t: torch.Tensor, n: int) -> bool:
+    """Whether two of the rows t[b, h, :n] have memory in common."""
+    (B, nkv), (s0, s1) = t.shape[:2], t.stride()[:2]
+    if (nkv == 1 or s1 >= n) and (B == 1 or s0 >= (nkv - 1) * s1 + n):
+        return False
+    return B * nkv > 1 and n > 0 and int(_starts(t).diff().min()) < n
+
+
+def _output_meets(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether a row of ``out`` has memory in common with any of ``t`` (of the same shape) but its own counterpart."""
+    (B, nkv, n), p, q = t.shape, out.data_ptr(), t.data_ptr()
+    a, b = out.stride(), t.stride()
+    if p == q and (B == 1 or a[0] == b[0]) and (nkv == 1 or a[1] == b[1]):
+        return False
+    if B * nkv * n == 0 or p >= q + 4 * ((B - 1) * b[0] + (nkv - 1) * b[1] + n) \
+            or q >= p + 4 * ((B - 1) * a[0] + (nkv - 1) * a[1] + n):
+        return False
+    x, y = _starts(out), _starts(t)
+    return bool((torch.searchsorted(y, x + n) > torch.searchsorted(y, x - n, right=True)).any())
+
+
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a copy of it if not every row of the last dimension (a multiple of 64 two-byte elements) starts on a
     16-byte boundary."""
@@ -201,7 +229,7 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
     ``budget - recent`` of largest ``weights[B, nkv, W]`` among the others (ties: the lower slot); a shorter one keeps
     all of them.  The new pages must not be pages that this call reads.  Returns ``(new_lens[B], kept[B, nkv, budget],
     weights_out[B, nkv, W])``: the lengths afterwards, the slots kept (-1 behind the last one) and their weights (zeros
-    behind the last; ``weights_out`` may be ``weights`` itself)."""
+    behind the last; ``weights_out`` may be ``weights`` itself, else its rows lie apart from those of ``weights``)."""
     c, nkv, page, _, B, width = _cache(k_cache, v_cache, block_table)
     _accumulator(weights, B, nkv, width * page)
     if not (width * page <= EVICT_MAX_SLOTS):
@@ -219,6 +247,9 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
         if not (weights_out.shape == weights.shape and weights_out.dtype == torch.float32
                 and (weights.shape[2] <= 1 or weights_out.stride(2) == 1)):
             raise ValueError("weights_out must be float32 of the weights' shape")
+        if _rows_meet(weights_out, weights.shape[2]) or _output_meets(weights_out, weights):
+            raise ValueError("weights_out: rows must not be the same memory as each other or, but for `weights` itself, as "
+                             "rows of weights")
     _on_gpu(dev, k_cache, v_cache, block_table, lens, new_table, weights_out)
     new_lens = torch.empty_like(lens)
     kept = lens.new_empty((B, nkv, budget))
