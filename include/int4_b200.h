@@ -329,7 +329,8 @@ size_t i4b_paged_attention_workspace_size(int64_t seqs, int64_t nq, int64_t kv_h
  * kv head h / (nq / kv_heads), nq / kv_heads <= 1024; zeros where no slot is left.  fp32 softmax; for the product with
  * V the probabilities are sums of two values of the cache's type.  q: element (b, h, d) at q + b * stride_qb + h * stride_qh + d, strides multiples of 8,
  * 16-byte aligned.  weights, when not NULL: fp32, weights[b * stride_wb + kvh * stride_wh + j] += the probability of
- * slot j summed over the query heads of kv head kvh, j < lens[b]; the rest is left as it was.  Results repeat bit by
+ * slot j summed over the query heads of kv head kvh, j < lens[b]; the rest is left as it was.  Its rows of
+ * max_pages * page_size values must not have memory in common.  Results repeat bit by
  * bit for the same lengths.  workspace: 16-byte aligned. */
 int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int64_t stride_qb, int64_t stride_qh,
                                int64_t nq, const int32_t* lens, float scale, void* out, float* weights,

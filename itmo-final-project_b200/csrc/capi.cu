@@ -644,6 +644,7 @@ int i4b_paged_decode_attention(const i4b_paged_cache* cache, const void* q, int6
   if (nq == 1) stride_qh = 0;
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || stride_qb < 0 || stride_qh < 0 || stride_qb % 8 != 0 || stride_qh % 8 != 0)
     return I4B_ERR_LAYOUT;
+  if (weights && rows_meet(c, stride_wb, stride_wh, c.capacity)) return I4B_ERR_LAYOUT;
   DevInfo d;
   if (int st = current_device_info(&d)) return st;
   PagedAttnWorkspace w;

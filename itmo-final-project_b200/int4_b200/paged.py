@@ -198,6 +198,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     _indices(lens, "lens", B)
     if weights is not None:
         _accumulator(weights, B, nkv, width * page)
+        if _rows_meet(weights, width * page):
+            raise ValueError("weights of different sequences or kv heads must not be the same memory")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:

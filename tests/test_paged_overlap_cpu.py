@@ -71,3 +71,29 @@ def test_c_evict_refuses_rows_that_overlap():
 
     for sb, sh in ((96, 0), (0, 48), (96, 47), (47, 96), (-47, 96), (96, -1)):
         assert evict(sb, sh) == 4, (sb, sh)
+
+
+def _attend(weights):
+    k, v, table, lens = _tensors()
+    return int4_b200.paged_decode_attention(torch.zeros(B, 4, 64, dtype=torch.bfloat16), k, v, table, lens, weights=weights)
+
+
+@pytest.mark.parametrize("which", list(_shared_rows()))
+def test_attention_refuses_weights_whose_rows_share_memory(which):
+    with pytest.raises(ValueError, match="same memory"):
+        _attend(_shared_rows()[which])
+
+
+def test_attention_takes_weights_whose_rows_lie_apart():
+    wide = torch.zeros(B, NKV, SLOTS + 40)
+    slack = _buffer().as_strided((B, NKV, SLOTS + 8), (NKV * SLOTS, SLOTS, 1))  # rows as long as the tables' slots do not meet
+    for w in (wide, wide[..., 3:], torch.zeros(NKV, B, SLOTS).transpose(0, 1), torch.zeros(SLOTS * 4).as_strided((B, NKV, SLOTS), (SLOTS, 2 * SLOTS, 1)), slack):
+        with pytest.raises(ValueError, match="GPU only|one device"):
+            _attend(w)
+
+
+def test_c_attention_refuses_weights_that_overlap():
+    L = _lib.lib()
+    c = _lib.PAGED_CACHE.pack(0x1000, 0x2000, 2048, 1024, 64, 2048, 1024, 64, 0x3000, 3, 6, 2, 16, 64, 2, 3, 1)
+    for sb, sh in ((96, 0), (0, 48), (96, 47), (47, 96)):
+        assert L.i4b_paged_decode_attention(c, 0x4000, 512, 64, 8, 0x5000, 0.125, 0x6000, 0x8000, sb, sh, 0x7000, 1 << 40, None) == 4
