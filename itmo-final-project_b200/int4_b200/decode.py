@@ -629,9 +629,9 @@ class LlamaTP:
             h = h + self._all_reduce(L["down"](F.silu(g) * u))
         cache.lengths[seq] += S
         cache.seen[seq] += S
-        cache.lens[seq] += S
-        cache.positions[seq] += S
-        cache.live[seq] = 1
+        cache.lens[seq].add_(S)
+        cache.positions[seq].add_(S)
+        cache.live[seq].fill_(1)
         return self._head(h if all_logits else h[:, -1:])
 
     @torch.no_grad()

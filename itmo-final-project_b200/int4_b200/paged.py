@@ -265,13 +265,22 @@ def paged_evict(weights: torch.Tensor, lens: torch.Tensor, block_table: torch.Te
     return new_lens, kept, weights_out
 
 
+def _upload(values: list, device: torch.device) -> torch.Tensor:
+    """Whole numbers as an int64 tensor on the device, behind what its stream holds already: the host does not wait (torch
+    keeps the pinned copy until the transfer has run)."""
+    t = torch.tensor(values, dtype=torch.int64)
+    return t if device.type == "cpu" else t.pin_memory().to(device, non_blocking=True)
+
+
 class PagedKVCache:
     """Keys and values of up to ``max_seqs`` sequences, of up to ``max_len`` slots each, in pages of every layer.
 
     ``k[layer]`` / ``v[layer]`` are ``[num_pages, kv_heads, page_size, head_dim]``; one block table serves all layers.
     ``lens`` counts a sequence's slots, ``positions`` the tokens that it has seen (its next rotary position); they
     differ once something was evicted; ``max_positions`` bounds them (the rotary tables' length).  Which pages are free is kept on the host; the tensors that the kernels read
-    (``table``, ``lens``, ``positions``, ``live``) keep their addresses, so a captured step stays valid.  With
+    (``table``, ``lens``, ``positions``, ``live``) keep their addresses, so a captured step stays valid.
+    The host waits for nothing: what it changes in those tensors is queued on the current stream, which has to be the one
+    that the steps (or their graphs' replays) run on, or be ordered before them.  With
     ``track_weights`` every decode step adds the attention weights up in ``weights[layer]`` ``[max_seqs, kv_heads,
     slots]`` and ``evict`` can bound the sequences.  ``decode.LlamaTP.paged_cache`` builds one for a model."""
 
@@ -313,11 +322,14 @@ class PagedKVCache:
         missing = {seq: self._missing(seq, n) for seq, n in want.items()}
         if sum(missing.values()) > len(self.free_pages):
             raise _lib.Int4B200Error(f"paged cache: {sum(missing.values())} pages wanted, {len(self.free_pages)} free")
+        new = []
         for seq, m in missing.items():
-            if m:
-                at = len(self.pages[seq])
-                self.pages[seq] += [self.free_pages.pop() for _ in range(m)]
-                self.table[seq, at:at + m] = torch.tensor(self.pages[seq][at:], dtype=torch.int32).to(self.table.device)
+            at = len(self.pages[seq])
+            self.pages[seq] += [self.free_pages.pop() for _ in range(m)]
+            new += [(seq, at + i, page) for i, page in enumerate(self.pages[seq][at:])]
+        if new:
+            rows, columns, pages = _upload(new, self.table.device).unbind(1)
+            self.table.index_put_((rows, columns), pages.to(torch.int32))
 
     def reserve_step(self) -> None:
         """Host side of a decode step: a slot for every live sequence (before the step, or before its graph replays)."""
@@ -332,9 +344,9 @@ class PagedKVCache:
         _need(0 <= seq < self.max_seqs, f"sequence {seq} of a cache for {self.max_seqs}")
         self.free_pages += reversed(self.pages[seq])
         self.pages[seq], self.lengths[seq], self.seen[seq] = [], 0, 0
-        self.table[seq] = -1
+        self.table[seq].fill_(-1)  # (assigning a number to an element copies it from the host and waits)
         for t in (self.lens, self.positions, self.live):
-            t[seq] = 0
+            t[seq].fill_(0)
         if self.weights is not None:
             self.weights[:, seq].zero_()
 
@@ -350,7 +362,7 @@ class PagedKVCache:
             if need > len(self.free_pages):
                 raise _lib.Int4B200Error(f"paged cache: eviction of sequence {seq} wants {need} pages, {len(self.free_pages)} free")
             fresh = [self.free_pages.pop() for _ in range(need)]
-            new_table = torch.tensor([fresh], dtype=torch.int32).to(self.table.device)
+            new_table = _upload([fresh], self.table.device).to(torch.int32)
             row = slice(seq, seq + 1)
             for layer in range(self.k.shape[0]):
                 w = self.weights[layer, row]
@@ -358,7 +370,7 @@ class PagedKVCache:
                             recent=recent, weights_out=w)
             self.free_pages += reversed(self.pages[seq])
             self.pages[seq], self.lengths[seq] = fresh, budget
-            self.table[seq, need:] = -1
+            self.table[seq, need:].fill_(-1)
             self.table[row, :need] = new_table
-            self.lens[seq] = budget
+            self.lens[seq].fill_(budget)
         return cut

@@ -34,3 +34,37 @@ def test_tokens_of_rows_without_a_sequence_are_not_read(model):
         got = model.decode_paged(tok, caches[1])
         assert torch.isfinite(got).all() and torch.equal(got[1:3], want[1:3])
         assert tok[0, 0] == pad  # the caller's tensor is left as it is
+
+
+@torch.no_grad()
+def test_the_host_does_not_wait_for_the_gpu(model):
+    """Prompts, steps that take new pages, an eviction and a freed sequence, under torch's check for synchronising calls."""
+
+    def run(cache):
+        model.prefill_paged(prompts[0], cache, 0)
+        model.prefill_paged(prompts[1][:, :13], cache, 2)
+        model.prefill_paged(prompts[1][:, 13:], cache, 2)
+        out = [model.decode_paged(tok, cache) for _ in range(20)]
+        cache.evict(24, recent=4)
+        out.append(model.decode_paged(tok, cache))
+        cache.free(0)
+        model.prefill_paged(prompts[0], cache, 1)
+        out.append(model.decode_paged(tok, cache))
+        return torch.stack([x[2] for x in out])
+
+    prompts, tok = [_ids(23, 3), _ids(30, 4)], torch.ones(3, 1, dtype=torch.long, device="cuda")
+    caches = [model.paged_cache(40, max_seqs=3, page_size=8, max_len=96, track_weights=True) for _ in range(2)]
+    want = run(caches[0])  # what is set up by the first calls may wait
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        got = run(caches[1])
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(got, want)
+    a, b = caches
+    assert a.pages == b.pages and a.lengths == b.lengths == b.lens.tolist() and a.seen == b.seen == b.positions.tolist()
+    assert b.live.tolist() == [0, 1, 1] and torch.equal(a.table, b.table) and torch.equal(a.weights, b.weights)
+    for seq in range(3):
+        n = len(b.pages[seq])
+        assert b.table[seq].tolist() == b.pages[seq] + [-1] * (b.table.shape[1] - n)
