@@ -694,7 +694,8 @@ class LlamaTP:
                 add_rmsnorm(cur, delta, L["ln1"], x, self.eps)
                 qkv = L["qkv"](x)
             attend(i, qkv, att)
-            fused_ar = fold and self.peers is not None and self.matmul_allreduce
+            # (a paged step may have more rows than the exchange buffers, which hold max_batch of them: those are NCCL's)
+            fused_ar = fold and self.peers is not None and self.matmul_allreduce and B * self.hidden <= self.peers.capacity
             if fused_ar:
                 o = self._matmul_allreduce_or_none(att, L["o"].q)
                 fused_ar = o is not None
