@@ -142,34 +142,48 @@ def test_one_graph_with_and_without_shared_runs(cuda_device, with_weights):
             _check(out, w, q, k, v, table, lens)
 
 
+def _pairs(dtype, B, nkv, page, width, gen, device):
+    """Scores and values of rows of two slots: probabilities 1 and p relative to the larger, values round(p) and -1."""
+    s = torch.empty(B * width, nkv, page, device=device).uniform_(0.5, 1.5, generator=gen).to(dtype)
+    s[:, :, 1::2] = (s[:, :, 0::2].float() - torch.empty_like(s[:, :, 1::2], dtype=torch.float32).uniform_(0.05, 0.6, generator=gen)).to(dtype)
+    v = torch.full_like(s, -1)
+    v[:, :, 0::2] = (s[:, :, 1::2].double() - s[:, :, 0::2].double()).exp().to(dtype)
+    return s, v
+
+
+def _pair_reference(s, v, dtype):
+    """Outputs of rows of two slots in 64 bits, and the bound of an output's error.
+
+    Scores are exact and below 1.5: a probability is off by the roundings of three numbers below 2.2 (units of log 2) and by
+    2^-22 of the exponential, 2^-20 in all, and so is the sum; 8 half steps for the four sums and products."""
+    half = torch.finfo(dtype).eps / 2
+    p = torch.softmax(s.double(), -1)
+    ref = (p * v.double()).sum(-1)
+    return ref, half * ref.abs() + half * half + 2 * 2 ** -20 + 8 * STEP + torch.finfo(dtype).smallest_normal * half
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dim,G,width", [(64, 4, 4), (64, 16, 40), (128, 8, 4), (128, 16, 40)])
 def test_probabilities_have_two_values(cuda_device, dtype, dim, G, width):
-    """Values of +1 and -1 whose probabilities almost cancel: an output far below sum p |v|, which a probability rounded
-    once to the cache's type (off by up to ``half`` of itself) would miss.
-
-    Keys have one number that is not 0, so a score below 1.5 is exact and its exponential off by a few roundings of 2.2 and
-    2^-22: eps = 2^-20."""
+    """Values that leave of an output what rounding leaves of a probability: one rounded once to the cache's type would
+    give 0 (shown for the oracle at the end)."""
     import int4_b200
 
     gen = torch.Generator(device="cuda").manual_seed(dim + G)
-    page, B, nkv = 16, 3, 2
+    page, B, nkv = 16, 96, 2
+    s, sign = _pairs(dtype, B, nkv, page, width, gen, "cuda")
     k = torch.zeros(B * width, nkv, page, dim, device="cuda", dtype=dtype)
-    v = torch.ones_like(k)
-    k[..., 3] = torch.empty(k.shape[:3], device="cuda").uniform_(-1.5, 1.5, generator=gen).to(dtype)
-    # pairs of slots: the second has the first's score but for one step of the type, and the opposite value
-    k[:, :, 1::2, 3] = (k[:, :, 0::2, 3].float() * (1 + torch.finfo(dtype).eps)).to(dtype)
-    v[:, :, 1::2] = -1
+    k[..., 3] = s
+    v = sign[..., None].expand(k.shape).contiguous()
     table = torch.randperm(B * width, device="cuda", generator=gen).to(torch.int32).view(B, width)
-    lens = torch.tensor([width * page, 2, width * page - 6], device="cuda", dtype=torch.int32)
+    lens = torch.full((B,), 2, device="cuda", dtype=torch.int32)
     q = torch.zeros(B, nkv * G, dim, device="cuda", dtype=dtype)
     q[..., 3] = 1
     out = int4_b200.paged_decode_attention(q, k, v, table, lens, scale=1.0)
-    half = torch.finfo(dtype).eps / 2
-    for b, n in enumerate(lens.tolist()):
-        s = k[table[b].long(), :, :, 3].transpose(0, 1).reshape(nkv, -1)[:, :n].double()
-        p = torch.softmax(s, -1)
-        ref = (p * v[table[b].long(), :, :, 0].transpose(0, 1).reshape(nkv, -1)[:, :n].double()).sum(-1)
-        tol = half * ref.abs() + half * half + 2 * 2 ** -20 + 512 * STEP + n * 2.0 ** -51 + torch.finfo(dtype).smallest_normal * half
-        err = (out[b].view(nkv, G, dim).double() - ref[:, None, None]).abs()
-        assert (err <= tol[:, None, None]).all(), (b, float(err.max()), float(tol.max()))
+    ss, vv = (x[table[:, 0].long(), :, :2] for x in (s, sign))
+    ref, tol = _pair_reference(ss, vv, dtype)
+    err = (out.view(B, nkv, G, dim).double() - ref[:, :, None, None]).abs()
+    assert (err <= tol[:, :, None, None]).all(), (float(err.max()), float(tol.max()))
+    p = (ss.double() - ss.double().amax(-1, keepdim=True)).exp()
+    once = (p.to(dtype).double() * vv.double()).sum(-1) / p.sum(-1)
+    assert ((once - ref).abs() > 4 * tol).float().mean() > 0.25
