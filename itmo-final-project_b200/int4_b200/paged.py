@@ -104,6 +104,8 @@ def _rows_meet(t: torch.Tensor, n: int) -> bool:
     (B, nkv), (s0, s1) = t.shape[:2], t.stride()[:2]
     if (nkv == 1 or s1 >= n) and (B == 1 or s0 >= (nkv - 1) * s1 + n):
         return False
+    if (B == 1 or s0 >= n) and (nkv == 1 or s1 >= (B - 1) * s0 + n):
+        return False
     return B * nkv > 1 and n > 0 and int(_starts(t).diff().min()) < n
 
 
