@@ -320,14 +320,16 @@ int i4b_paged_kv_append(const i4b_paged_cache* cache, const void* qkv, int64_t s
                         const int32_t* positions, const int32_t* slots, const int32_t* seqs, void* q_out, void* stream);
 
 /* Bytes of workspace i4b_paged_decode_attention needs: 0 for tables of up to 256 slots (128 at head_dim 128) without
- * weights (and for sizes that are not supported, or without a B200).  Needs no clearing; calls that share a workspace
+ * weights (and for sizes that are not supported, or without a B200); with weights 4 * seqs * nq * capacity bytes and
+ * some MB, whatever the lengths are.  Needs no clearing; calls that share a workspace
  * must not overlap in time. */
 size_t i4b_paged_attention_workspace_size(int64_t seqs, int64_t nq, int64_t kv_heads, int64_t head_dim,
                                           int64_t capacity, int with_weights);
 
 /* out[seqs, nq, head_dim] = softmax(q . K^T * scale) . V over slots 0..lens[b]-1 of each sequence, query head h reading
  * kv head h / (nq / kv_heads), nq / kv_heads <= 1024; zeros where no slot is left.  fp32 softmax; for the product with
- * V the probabilities are sums of two values of the cache's type.  q: element (b, h, d) at q + b * stride_qb + h * stride_qh + d, strides multiples of 8,
+ * V the probabilities are sums of two values of the cache's type, in fp16 scaled: within 2^-16 (bf16) or 2^-22 (fp16, or
+ * 2^-51 absolutely) of themselves.  A NaN or infinite value within a length makes its outputs NaN or infinite.  q: element (b, h, d) at q + b * stride_qb + h * stride_qh + d, strides multiples of 8,
  * 16-byte aligned.  weights, when not NULL: fp32, weights[b * stride_wb + kvh * stride_wh + j] += the probability of
  * slot j summed over the query heads of kv head kvh, j < lens[b]; the rest is left as it was.  Its rows of
  * max_pages * page_size values must not have memory in common.  Results repeat bit by

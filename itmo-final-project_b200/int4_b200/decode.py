@@ -588,7 +588,8 @@ class LlamaTP:
     def score(self, ids: torch.Tensor, top: int = 0):
         """Log probabilities of the tokens ids[B, S] given those before them, ``token_logprobs`` of positions 1..S-1:
         ``(logprobs, entropy, top_logprobs, top_ids)``, [B, S - 1] and [B, S - 1, top].  The mean of ``-logprobs`` is
-        the reference's token NLL (``eval_ppl``, ``benchmarks/eval_llama.py:77-117``).  Overwrites the static cache."""
+        the reference's token NLL (``eval_ppl``, ``benchmarks/eval_llama.py:77-117``).  Overwrites the static cache.
+        With more than one sequence the logits are copied once, to leave out the last position's."""
         logits = self.prefill(ids, all_logits=True)
         return token_logprobs(logits[:, :-1], ids[:, 1:], top)
 

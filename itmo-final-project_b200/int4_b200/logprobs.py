@@ -19,7 +19,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0):
     vocabulary a NaN).  ``entropy[...]``: -sum p log p.  ``top_logprobs`` / ``top_ids`` ``[..., top]``: the ``top``
     largest logits of each row in order, ties to the lower index (None when ``top`` is 0; at most 32).  float32,
     ids int64.  -inf logits have probability 0; a row of nothing else has log probabilities -inf and entropy 0; a NaN
-    or +inf makes the row's numbers NaN.  The logits are read once, on the current stream; no backward pass."""
+    or +inf makes the row's numbers NaN.  The logits are read once, on the current stream; no backward pass.
+    Logits that are not rows one stride apart (``x[:, :-1]`` of a batch) or whose last dimension is strided are copied
+    first."""
     if logits.dtype not in _lib.DTYPE_CODE or logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError("logits must be [..., vocabulary] in bfloat16, float16 or float32")
     lead, V = logits.shape[:-1], logits.shape[-1]

@@ -189,7 +189,12 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     ``scale`` is head_dim ** -0.5 unless given.  ``weights`` (float32 ``[B, nkv, >= pages * page_size]``) is added to
     in place: slot j of a sequence gets its probability summed over the query heads of the kv head, which is what
-    ``paged_evict`` selects by.  Lengths are clamped to what the block table's rows can hold."""
+    ``paged_evict`` selects by.  Lengths are clamped to what the block table's rows can hold.  A NaN or infinite value
+    within a length makes its outputs NaN or infinite.
+
+    The call takes workspace from torch's allocator.  With ``weights`` that holds a float32 score for every slot that the
+    table can name, ``4 * B * nq * pages * page_size`` bytes whatever the lengths are (32 sequences of 32 heads and 131072
+    slots: 537 MB); a captured graph keeps it."""
     c, nkv, page, dim, B, width = _cache(k_cache, v_cache, block_table)
     shape = q.shape
     if len(shape) != 3 or shape[0] != B or shape[2] != dim or q.dtype is not k_cache.dtype:
@@ -281,6 +286,9 @@ class PagedKVCache:
     ``lens`` counts a sequence's slots, ``positions`` the tokens that it has seen (its next rotary position); they
     differ once something was evicted; ``max_positions`` bounds them (the rotary tables' length).  Which pages are free is kept on the host; the tensors that the kernels read
     (``table``, ``lens``, ``positions``, ``live``) keep their addresses, so a captured step stays valid.
+    ``weights`` takes ``4 * layers * max_seqs * kv_heads`` bytes per slot of ``max_len``, and a step's workspace grows with
+    ``max_seqs * max_len`` too (``paged_decode_attention``), whatever ``num_pages`` is.  A prompt adds nothing to the
+    weights: slots are ranked by the steps that followed, and before any step all of them weigh 0.
     The host waits for nothing: what it changes in those tensors is queued on the current stream, which has to be the one
     that the steps (or their graphs' replays) run on, or be ordered before them.  With
     ``track_weights`` every decode step adds the attention weights up in ``weights[layer]`` ``[max_seqs, kv_heads,
@@ -354,8 +362,10 @@ class PagedKVCache:
 
     def evict(self, budget: int, recent: int = 0) -> list[int]:
         """Cut every sequence of more than ``budget`` slots to the ``recent`` last and the ones of highest accumulated
-        weight (``paged_evict``, per layer and kv head); returns the sequences that were cut.  Needs free pages for the
-        kept slots of one sequence at a time; the old pages are free afterwards."""
+        weight (``paged_evict``, per layer and kv head); returns the sequences that were cut.  Slots that no decode step
+        has attended weigh 0, and of equal weights the lower slots stay: right after a prompt, its beginning.  Needs free
+        pages for the kept slots of one sequence at a time, or raises before the first is cut (a cut gives back at least
+        as many as it takes)."""
         _need(self.weights is not None, "evict needs a cache with track_weights")
         _need(budget >= 1 and 0 <= recent <= budget, f"budget {budget} and recent {recent}: 0 <= recent <= budget, budget >= 1")
         cut = [seq for seq in range(self.max_seqs) if self.lengths[seq] > budget]
