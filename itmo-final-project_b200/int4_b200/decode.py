@@ -639,8 +639,9 @@ class LlamaTP:
     def decode_paged(self, ids: torch.Tensor, cache: PagedKVCache, reserve: bool = True) -> torch.Tensor:
         """One token for every sequence of ``cache``, each at its own position: ids[max_seqs, 1], logits
         [max_seqs, 1, V].  Rows of sequences that are not live are computed and mean nothing, whatever their ids (-1
-        will do); their cache stays as it is.  ``reserve=False`` leaves the host side to the caller (``cache.reserve_step()``): the rest has no host
-        synchronisation, keeps its addresses and can be captured in a CUDA graph."""
+        will do); their cache stays as it is.  ``reserve=False`` leaves the host side to the caller
+        (``cache.reserve_step()``): the rest has no host synchronisation, keeps its addresses and can be captured in a
+        CUDA graph."""
         assert self.fused, "the paged decode step runs the fused kernels"
         assert ids.shape == (cache.max_seqs, 1), (tuple(ids.shape), cache.max_seqs)
         if reserve:
